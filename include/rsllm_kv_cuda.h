@@ -662,6 +662,125 @@ RKV_API rkv_status rkv_indexer_topk_f32(const float* rows, const int64_t* row_st
                                         float* scores, int64_t ld, int32_t* out_idx, uint32_t* d_status,
                                         rkv_stream_t stream);
 
+/* ---- grouped-head (GQA) paged KV cache --------------------------------------
+ * The paged cache of a model with separate K and V heads (rsLLM plans its paged
+ * layout for every attention form, docs/03-HLD.md:363-369; its models today are
+ * MLA only, so these entry points have no rsLLM counterpart).  Pages hold 64
+ * tokens, as in the MLA pool, so the same page tables, slots, allocator and
+ * prefix store serve both (a plan-only pool, RKV_PLAN_ONLY, plans the pages; its
+ * moves are applied with rkv_gqa_copy_pages).
+ *
+ * A view: n_layers regions of n_pages pages; page p of layer l holds, for K and
+ * then for V, [n_kv_heads][64 rows][head_dim] elements, so the whole cache is one
+ * array [n_layers][n_pages][2][n_kv_heads][64][head_dim] at base (256-byte
+ * aligned).  head_dim is 64 or 128.  The reads below never look at rows past a
+ * sequence's length, whatever they hold.
+ *
+ * Rows of q, k and v are given as a pointer, a token stride and a head stride
+ * in elements (the head_dim elements of a row are contiguous), so that views
+ * of one fused projection need no copy: pointers 16-byte aligned, strides
+ * multiples of 8.  n_q_heads is a multiple of n_kv_heads, at most 64 times as
+ * many; q head h reads kv head h / (n_q_heads / n_kv_heads). */
+#define RKV_GQA_BF16 0
+#define RKV_GQA_F16 1
+#define RKV_GQA_MAX_GROUP 64
+typedef struct rkv_gqa_view {
+  void* base;
+  int64_t n_pages; /* pages per layer; slots are < n_pages * 64 */
+  int32_t n_layers;
+  int32_t n_kv_heads;
+  int32_t head_dim; /* 64 or 128 */
+  int32_t dtype;    /* RKV_GQA_BF16 or RKV_GQA_F16: of the cache, q, k, v and outputs */
+} rkv_gqa_view;
+
+/* Bytes of one page and of a whole cache. */
+RKV_API int64_t rkv_gqa_page_bytes(int32_t n_kv_heads, int32_t head_dim);
+RKV_API int64_t rkv_gqa_bytes(const rkv_gqa_view* cache);
+
+/* Rotary positions: the first rot_dim lanes of a row are rotated in pairs --
+ * lanes (i, i + rot_dim / 2), or (2 i, 2 i + 1) if interleaved -- by the angle
+ * whose cosine and sine are table[pos][i].  With several axes (time, height,
+ * width of an image or video token) pair i takes its position from the axis
+ * whose section it falls into: the first section[0] pairs from axis 0, the
+ * next section[1] from axis 1, and so on. */
+typedef struct rkv_gqa_rotary {
+  const float* table; /* device f32 [table_rows][rot_dim / 2][2]: cosine, sine; 16-byte aligned */
+  int64_t table_rows;
+  int32_t rot_dim;     /* a multiple of 16, at most head_dim */
+  int32_t interleaved; /* 0 or 1 */
+  int32_t n_axes;      /* 1 to 4 */
+  int32_t section[4];  /* pairs of each axis, sum rot_dim / 2 */
+} rkv_gqa_rotary;
+
+/* Stores the K and V rows of n_tokens new tokens in one layer of the cache,
+ * token t at slot slot_mapping[t] (int32, negative: not stored).  With rotary
+ * (else NULL) k is rotated on its way, and q, if given, is rotated into q_out
+ * (contiguous [n_tokens][n_q_heads][head_dim]; it may be q itself where q is
+ * contiguous).  pos: device int32 [n_axes][n_tokens].  Products and sums are
+ * f32, rounded once.
+ * Device status, per row: a slot >= n_pages * 64, or a position outside
+ * [0, table_rows) (that token's rows are not stored and its q_out is zero), sets
+ * INDEX_OUT_OF_RANGE; a K or V row with a value that is not finite, as
+ * stored, sets NON_FINITE_INPUT and is not written. */
+RKV_API rkv_status rkv_gqa_append(const rkv_gqa_view* cache, int32_t layer, const void* k, int64_t k_token_stride,
+                                  int64_t k_head_stride, const void* v, int64_t v_token_stride, int64_t v_head_stride,
+                                  int64_t n_tokens, const int32_t* slot_mapping, const rkv_gqa_rotary* rotary,
+                                  const int32_t* pos, const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                                  int32_t n_q_heads, void* q_out, uint32_t* d_status, rkv_stream_t stream);
+
+/* rkv_copy_pages for this cache: for every layer, page dst[i] <- page src[i],
+ * i < n; the src and dst sets must be disjoint and no page twice in dst.  Ids
+ * outside [0, n_pages) set INDEX_OUT_OF_RANGE and skip that pair. */
+RKV_API rkv_status rkv_gqa_copy_pages(const rkv_gqa_view* cache, const int32_t* src, const int32_t* dst, int64_t n,
+                                      uint32_t* d_status, rkv_stream_t stream);
+
+/* Causal attention of packed new tokens over the cache: sequence s has the
+ * tokens [cu_q[s], cu_q[s + 1]) of q (int32 [n_seq + 1], ascending from 0) and
+ * kv_lens[s] rows in its pages (page_table int32 [n_seq][pt_stride], one entry
+ * per 64 rows), the new tokens' own rows, appended before, being the last ones:
+ * its i-th new token sits at position p = kv_lens[s] - q_len + i and sees the
+ * rows j <= p, with window > 0 only those with j > p - window.
+ * out[t][h] = sum_j softmax_j(q . k_j * softmax_scale) v_j, in the cache's
+ * type (contiguous [n_tokens][n_q_heads][head_dim], 16-byte aligned); sinks
+ * (f32 [n_q_heads] or NULL) add exp(sink) to a head's denominator.  A token that
+ * sees no row gives zeros.
+ * softmax_scale must be finite and > 0.
+ * Device status: a page id outside the pool sets INDEX_OUT_OF_RANGE and reads
+ * as zero rows; a length or offset outside the tables sets it too and is cut to
+ * what they hold.
+ * n_splits: each token's rows are cut into n_splits ranges that are processed in
+ * parallel and joined through workspace (rkv_gqa_prefill_workspace_bytes bytes of
+ * device memory, 16-byte aligned; may be NULL when n_splits == 1): for few new
+ * tokens behind a long cached prefix.  rkv_gqa_prefill_splits says how many fill
+ * the GPU (1 where the tokens alone do).
+ * Numerics: logits and sums are f32; the weights are rounded to the cache's type
+ * before their product with V, as the tensor cores take them.  A K or V row that
+ * is not finite (rkv_gqa_append stores none) makes the tokens that see it NaN
+ * and may do so to earlier tokens of its sequence. */
+RKV_API int32_t rkv_gqa_prefill_splits(const rkv_gqa_view* cache, int64_t n_tokens, int32_t n_q_heads, int32_t n_seq,
+                                       int64_t pt_stride);
+RKV_API int64_t rkv_gqa_prefill_workspace_bytes(const rkv_gqa_view* cache, int64_t n_tokens, int32_t n_q_heads,
+                                                int32_t n_splits);
+RKV_API rkv_status rkv_gqa_prefill(const rkv_gqa_view* cache, int32_t layer, const void* q, int64_t q_token_stride,
+                                   int64_t q_head_stride, int64_t n_tokens, int32_t n_q_heads, const int32_t* cu_q,
+                                   int32_t n_seq, const int32_t* page_table, int64_t pt_stride,
+                                   const int32_t* kv_lens, int32_t window, const float* sinks, float softmax_scale,
+                                   int32_t n_splits, void* workspace, void* out, uint32_t* d_status,
+                                   rkv_stream_t stream);
+
+/* Attention of one new token per sequence over the cache: rkv_gqa_prefill with
+ * one token in each sequence (q and out [n_seq][n_q_heads][head_dim], the token
+ * at position kv_lens[s] - 1; a sequence of no rows gives zeros), the rows
+ * divided evenly over the GPU whatever the lengths and joined through workspace
+ * (rkv_gqa_decode_workspace_bytes bytes of device memory, 16-byte aligned; its
+ * contents need no initialisation and do not outlast the call). */
+RKV_API int64_t rkv_gqa_decode_workspace_bytes(const rkv_gqa_view* cache, int32_t n_seq, int32_t n_q_heads);
+RKV_API rkv_status rkv_gqa_decode(const rkv_gqa_view* cache, int32_t layer, const void* q, int64_t q_token_stride,
+                                  int64_t q_head_stride, int32_t n_seq, int32_t n_q_heads, const int32_t* page_table,
+                                  int64_t pt_stride, const int32_t* kv_lens, int32_t window, const float* sinks,
+                                  float softmax_scale, void* workspace, void* out, uint32_t* d_status,
+                                  rkv_stream_t stream);
+
 /* ---- codec pin ---------------------------------------------------------------
  * out[i] = E4M3 code the append kernel stores for the f32 lane value whose
  * bit pattern is first_bits + i (already divided by its block scale), i < n:

@@ -60,6 +60,24 @@ class PoolStats(Structure):
                 ("tick", c_int64), ("high_water", c_int64)]
 
 
+class GqaView(Structure):
+    """``rkv_gqa_view``: a grouped-head cache."""
+
+    _fields_ = [("base", c_void_p), ("n_pages", c_int64), ("n_layers", c_int32), ("n_kv_heads", c_int32),
+                ("head_dim", c_int32), ("dtype", c_int32)]
+
+
+class GqaRotary(Structure):
+    """``rkv_gqa_rotary``."""
+
+    _fields_ = [("table", c_void_p), ("table_rows", c_int64), ("rot_dim", c_int32), ("interleaved", c_int32),
+                ("n_axes", c_int32), ("section", c_int32 * 4)]
+
+
+GQA_BF16, GQA_F16 = 0, 1
+GQA_MAX_GROUP = 64
+
+
 class KvcHeader(Structure):
     """``rkv_kvc_header``."""
 
@@ -130,6 +148,20 @@ SIGNATURES = {
                                          c_int32, _f32p, c_int64, _u32p, c_void_p]),
     "rkv_indexer_topk_f32": (c_int32, [_f32p, c_void_p, _i32p, c_int64, _f32p, _f32p, _i32p, _i32p, c_int32,
                                        c_int32, c_int32, _f32p, c_int64, _i32p, _u32p, c_void_p]),
+    "rkv_gqa_page_bytes": (c_int64, [c_int32, c_int32]),
+    "rkv_gqa_bytes": (c_int64, [c_void_p]),
+    "rkv_gqa_append": (c_int32, [c_void_p, c_int32, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int64,
+                                 _i32p, c_void_p, _i32p, c_void_p, c_int64, c_int64, c_int32, c_void_p, _u32p,
+                                 c_void_p]),
+    "rkv_gqa_copy_pages": (c_int32, [c_void_p, _i32p, _i32p, c_int64, _u32p, c_void_p]),
+    "rkv_gqa_prefill_splits": (c_int32, [c_void_p, c_int64, c_int32, c_int32, c_int64]),
+    "rkv_gqa_prefill_workspace_bytes": (c_int64, [c_void_p, c_int64, c_int32, c_int32]),
+    "rkv_gqa_prefill": (c_int32, [c_void_p, c_int32, c_void_p, c_int64, c_int64, c_int64, c_int32, _i32p, c_int32,
+                                  _i32p, c_int64, _i32p, c_int32, _f32p, c_float, c_int32, c_void_p, c_void_p, _u32p,
+                                  c_void_p]),
+    "rkv_gqa_decode_workspace_bytes": (c_int64, [c_void_p, c_int32, c_int32]),
+    "rkv_gqa_decode": (c_int32, [c_void_p, c_int32, c_void_p, c_int64, c_int64, c_int32, c_int32, _i32p, c_int64,
+                                 _i32p, c_int32, _f32p, c_float, c_void_p, c_void_p, _u32p, c_void_p]),
     "rkv_pool_create": (c_int32, [_P(PoolDesc), _P(c_void_p)]),
     "rkv_pool_destroy": (None, [c_void_p]),
     "rkv_pool_get_view": (c_int32, [c_void_p, _P(PoolView)]),
