@@ -3,6 +3,8 @@
 // whole-page copies.
 #include "rkv_gqa.cuh"
 
+#include <cmath>
+
 namespace rkv {
 namespace gqa {
 
@@ -39,6 +41,65 @@ rkv_status check_heads(const rkv_gqa_view* c, int32_t n_q_heads, const char* wha
                       "%s: n_q_heads must be a multiple of the %d kv heads, at most %d times as many; got %d", what,
                       c->n_kv_heads, RKV_GQA_MAX_GROUP, n_q_heads);
   return RKV_OK;
+}
+
+rkv_status check_attend(const AttendArgs& a, const char* what) {
+  rkv_status st = check_rows(a.q, a.q_ts, a.q_hs, "q", what);
+  if (st != RKV_OK) return st;
+  if (a.pt_stride < 1 || a.pt_stride > INT32_MAX / kPage)
+    return fail_shape("pt_stride", 1, a.pt_stride, "%s: pt_stride must be at least 1 and pt_stride * 64 fit in int32", what);
+  if (a.window < 0) return fail_shape("window", 0, a.window, "%s: window must not be negative", what);
+  if (!(a.scale > 0.f) || !std::isfinite(a.scale))
+    return fail(RKV_ERR_INVALID_ARGUMENT, "%s: softmax_scale must be finite and positive", what);
+  if (!a.page_table || !a.kv_lens || !a.out || !aligned(a.out, 16))
+    return fail(RKV_ERR_INVALID_ARGUMENT, "%s: page_table, kv_lens and a 16-byte aligned out are required", what);
+  return RKV_OK;
+}
+
+// ---- tensor maps ---------------------------------------------------------------------
+typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// The driver's encoder, looked up once (the library does not link the driver).
+static EncodeTiled encoder() {
+  static EncodeTiled fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &found) != cudaSuccess ||
+        found != cudaDriverEntryPointSuccess)
+      p = nullptr;
+    return reinterpret_cast<EncodeTiled>(p);
+  }();
+  return fn;
+}
+
+static rkv_status encode(const rkv_gqa_view& c, const void* base, int rank, const cuuint64_t* dims,
+                         const cuuint64_t* strides, const cuuint32_t* box, CUtensorMap* out, const char* what) {
+  const EncodeTiled fn = encoder();
+  if (!fn) return fail(RKV_ERR_CUDA, "%s: the driver has no cuTensorMapEncodeTiled", what);
+  const cuuint32_t step[3] = {1, 1, 1};
+  const CUresult r = fn(out, c.dtype == RKV_GQA_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                        rank, const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(RKV_ERR_CUDA, "%s: cuTensorMapEncodeTiled failed (%d)", what, (int)r);
+  return RKV_OK;
+}
+
+rkv_status cache_map(const rkv_gqa_view& c, CUtensorMap* out, const char* what) {
+  const cuuint64_t dims[2] = {(cuuint64_t)c.head_dim, (cuuint64_t)row_base(c, c.n_layers, 0, 0, 0)};
+  const cuuint64_t strides[1] = {(cuuint64_t)c.head_dim * 2};
+  const cuuint32_t box[2] = {64, kPage};
+  return encode(c, c.base, 2, dims, strides, box, out, what);
+}
+
+rkv_status q_map(const rkv_gqa_view& c, const void* q, int64_t token_stride, int64_t head_stride, int64_t n_tokens,
+                 int32_t n_heads, int box_tokens, int box_heads, CUtensorMap* out, const char* what) {
+  const cuuint64_t dims[3] = {(cuuint64_t)c.head_dim, (cuuint64_t)n_heads, (cuuint64_t)n_tokens};
+  const cuuint64_t strides[2] = {(cuuint64_t)head_stride * 2, (cuuint64_t)token_stride * 2};
+  const cuuint32_t box[3] = {64, (cuuint32_t)box_heads, (cuuint32_t)box_tokens};
+  return encode(c, q, 3, dims, strides, box, out, what);
 }
 
 // ---- rotary append ---------------------------------------------------------------

@@ -1,13 +1,11 @@
 // rkv_gqa_prefill.cu -- causal attention of packed new tokens over the
-// grouped-head paged cache, and of one new token per sequence.
+// grouped-head paged cache.
 //
 //   x_j = softmax_scale * q . k_j over the rows j that the token sees,
 //   out = sum_j exp(x_j - m) v_j / (sum_j exp(x_j - m) + exp(sink - m)).
 //
 // One warp per (token, q head), one pass over the rows with the running
 // maximum and sum; a lane holds head_dim / 32 lanes of q, k and v.
-#include <cmath>
-
 #include "rkv_gqa.cuh"
 
 namespace rkv {
@@ -20,7 +18,7 @@ struct AttendParams {
   int64_t q_ts, q_hs;
   int64_t n_tokens;
   int n_q_heads;
-  const int32_t* cu_q;  // NULL: one token per sequence
+  const int32_t* cu_q;
   int n_seq;
   const int32_t* page_table;
   int64_t pt_stride;
@@ -32,12 +30,6 @@ struct AttendParams {
   uint32_t* status;
 };
 
-__device__ __forceinline__ float exp2_fast(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 template <typename T, int D>
 __global__ void __launch_bounds__(128) attend_kernel(const AttendParams p) {
   constexpr int kWords = D / 64;  // words of two lanes each
@@ -46,22 +38,18 @@ __global__ void __launch_bounds__(128) attend_kernel(const AttendParams p) {
   const int64_t t = item / p.n_q_heads;
   const int h = (int)(item % p.n_q_heads);
   if (t >= p.n_tokens) return;
-  int seq = (int)t, q_len = 1, i = 0;
-  if (p.cu_q) {
-    int lo = 0, hi = p.n_seq;  // the last sequence that starts at or before t
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) / 2;
-      if (p.cu_q[mid] <= t) lo = mid;
-      else hi = mid;
-    }
-    seq = lo;
-    if (t < p.cu_q[seq] || t >= p.cu_q[seq + 1]) {
-      if (lane == 0) set_status(p.status, RKV_ERR_INDEX_OUT_OF_RANGE);
-      return;
-    }
-    q_len = p.cu_q[seq + 1] - p.cu_q[seq];
-    i = (int)(t - p.cu_q[seq]);
+  int seq = 0, hi = p.n_seq;  // the last sequence that starts at or before t
+  while (hi - seq > 1) {
+    const int mid = (seq + hi) / 2;
+    if (p.cu_q[mid] <= t) seq = mid;
+    else hi = mid;
   }
+  if (t < p.cu_q[seq] || t >= p.cu_q[seq + 1]) {
+    if (lane == 0) set_status(p.status, RKV_ERR_INDEX_OUT_OF_RANGE);
+    return;
+  }
+  const int q_len = p.cu_q[seq + 1] - p.cu_q[seq];
+  const int i = (int)(t - p.cu_q[seq]);
   int64_t len = p.kv_lens[seq];
   if (len < 0 || len > p.pt_stride * kPage) {
     if (lane == 0) set_status(p.status, RKV_ERR_INDEX_OUT_OF_RANGE);
@@ -102,7 +90,7 @@ __global__ void __launch_bounds__(128) attend_kernel(const AttendParams p) {
     for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
     x *= p.scale_log2;
     const float top = fmaxf(m, x);
-    const float old = m == -INFINITY ? 0.f : exp2_fast(m - top), e = exp2_fast(x - top);
+    const float old = m == -INFINITY ? 0.f : ex2(m - top), e = ex2(x - top);
     m = top;
     l = l * old + e;
 #pragma unroll
@@ -128,21 +116,6 @@ static rkv_status attend(const AttendParams& p, const char* what, cudaStream_t s
     else attend_kernel<F16, 128><<<(unsigned)blocks, 128, 0, s>>>(p);
   }
   return check_launch(what);
-}
-
-// What both attentions check; n_seq and n_tokens are positive.
-static rkv_status check_attend(const void* q, int64_t q_ts, int64_t q_hs, const int32_t* page_table, int64_t pt_stride,
-                               const int32_t* kv_lens, int32_t window, float scale, const void* out, const char* what) {
-  rkv_status st = check_rows(q, q_ts, q_hs, "q", what);
-  if (st != RKV_OK) return st;
-  if (pt_stride < 1 || pt_stride > INT32_MAX / kPage)
-    return fail_shape("pt_stride", 1, pt_stride, "%s: pt_stride must be at least 1 and pt_stride * 64 fit in int32", what);
-  if (window < 0) return fail_shape("window", 0, window, "%s: window must not be negative", what);
-  if (!(scale > 0.f) || !std::isfinite(scale))
-    return fail(RKV_ERR_INVALID_ARGUMENT, "%s: softmax_scale must be finite and positive", what);
-  if (!page_table || !kv_lens || !out || !aligned(out, 16))
-    return fail(RKV_ERR_INVALID_ARGUMENT, "%s: page_table, kv_lens and a 16-byte aligned out are required", what);
-  return RKV_OK;
 }
 
 }  // namespace gqa
@@ -180,44 +153,14 @@ extern "C" rkv_status rkv_gqa_prefill(const rkv_gqa_view* cache, int32_t layer, 
     clear_error();
     return RKV_OK;
   }
-  st = check_attend(q, q_token_stride, q_head_stride, page_table, pt_stride, kv_lens, window, softmax_scale, out, what);
+  const AttendArgs args = {*cache,     layer,   q,      q_token_stride, q_head_stride, n_tokens, n_q_heads, page_table,
+                           pt_stride,  kv_lens, window, sinks,          softmax_scale, out,      d_status};
+  st = check_attend(args, what);
   if (st != RKV_OK) return st;
   if (!cu_q) return fail(RKV_ERR_INVALID_ARGUMENT, "%s: cu_q is required", what);
   const AttendParams p = {*cache,    layer,      static_cast<const uint16_t*>(q),
                           q_token_stride, q_head_stride, n_tokens,
                           n_q_heads, cu_q,       n_seq,
-                          page_table, pt_stride, kv_lens,
-                          window,    sinks,      (float)((double)softmax_scale * 1.4426950408889634),
-                          static_cast<uint16_t*>(out), d_status};
-  return attend(p, what, (cudaStream_t)stream);
-}
-
-extern "C" int64_t rkv_gqa_decode_workspace_bytes(const rkv_gqa_view* cache, int32_t n_seq, int32_t n_q_heads) {
-  if (!cache || n_seq < 0 || n_q_heads < 1) return -1;
-  return 0;
-}
-
-extern "C" rkv_status rkv_gqa_decode(const rkv_gqa_view* cache, int32_t layer, const void* q, int64_t q_token_stride,
-                                     int64_t q_head_stride, int32_t n_seq, int32_t n_q_heads, const int32_t* page_table,
-                                     int64_t pt_stride, const int32_t* kv_lens, int32_t window, const float* sinks,
-                                     float softmax_scale, void* workspace, void* out, uint32_t* d_status,
-                                     rkv_stream_t stream) {
-  using namespace rkv;
-  using namespace rkv::gqa;
-  static const char* what = "rkv_gqa_decode";
-  rkv_status st = check_cache(cache, layer, what);
-  if (st != RKV_OK) return st;
-  if ((st = check_heads(cache, n_q_heads, what)) != RKV_OK) return st;
-  if (n_seq < 0) return fail_shape("n_seq", 0, n_seq, "%s: n_seq < 0", what);
-  if (n_seq == 0) {
-    clear_error();
-    return RKV_OK;
-  }
-  st = check_attend(q, q_token_stride, q_head_stride, page_table, pt_stride, kv_lens, window, softmax_scale, out, what);
-  if (st != RKV_OK) return st;
-  const AttendParams p = {*cache,    layer,      static_cast<const uint16_t*>(q),
-                          q_token_stride, q_head_stride, n_seq,
-                          n_q_heads, nullptr,    n_seq,
                           page_table, pt_stride, kv_lens,
                           window,    sinks,      (float)((double)softmax_scale * 1.4426950408889634),
                           static_cast<uint16_t*>(out), d_status};

@@ -389,6 +389,7 @@ def test_python_refusals(cuda):
         lambda: pool.decode(0, q, table, i32(5), window=-1),
         lambda: pool.decode(0, q, table, i32(5), sinks=torch.zeros(7, device=cuda)),
         lambda: pool.decode(0, q, table, i32(5), out=q[:, :4]),
+        lambda: pool.decode(0, q, table, i32(5), workspace=torch.zeros(8, device=cuda, dtype=torch.uint8)),
         lambda: pool.prefill(0, q, i32(0, 1, 1), table, i32(5)),
         lambda: pool.prefill(0, q, i32(0, 1), table, i32(5), n_splits=65),
         lambda: pool.prefill(0, torch.zeros((1, 8, 132), dtype=BF, device=cuda)[:, :, :128], i32(0, 1), table, i32(5)),
