@@ -1,23 +1,48 @@
 // rkv_gqa_prefill.cu -- causal attention of packed new tokens over the
 // grouped-head paged cache.
 //
-//   x_j = softmax_scale * q . k_j over the rows j that the token sees,
+//   x_j = softmax_scale * q . k_j over the rows j that a token sees,
 //   out = sum_j exp(x_j - m) v_j / (sum_j exp(x_j - m) + exp(sink - m)).
 //
-// One warp per (token, q head), one pass over the rows with the running
-// maximum and sum; a lane holds head_dim / 32 lanes of q, k and v.
+// 4 head_dim flops per (q head, token, visible row): the 5th-generation tensor
+// cores bound it, and close behind them the 16 exponentials a clock that an SM
+// evaluates (a 128 x 128 tile: 1024 clocks of each at head_dim 128).
+//
+// One CTA takes two tiles of 128 q rows of one kv head, against 128 key rows
+// at a time.  A tile's rows are the group's q heads of 128 / group
+// consecutive tokens, token by token, so that every K and V row fetched serves
+// the whole group and a tile of a long prompt has a short diagonal.
+//
+//   warps 0-3, 4-7  softmax of tile 0 and of tile 1, one row a thread: S from
+//                   tensor memory, running maximum and sum, P (in the cache's
+//                   type) back over S; the epilogue
+//   warp 8          issues S = Q K^T (Q, K in shared memory) and O += P V (P in
+//                   tensor memory, V in shared memory)
+//   warp 9          copies Q, K and V by tensor maps (two pages a tile, a ring
+//                   of stages)
+//
+// Tensor memory: S0, S1 (128 columns each, P over the first 64), O0, O1
+// (head_dim columns each).  The tensor cores work on one tile while the
+// softmax warps of the other are busy: O0 += P0 V, S0 = Q0 K' is followed by O1
+// += P1 V, S1 = Q1 K', each waiting only for its own tile's P.
+#include <atomic>
+
 #include "rkv_gqa.cuh"
 
 namespace rkv {
 namespace gqa {
+namespace pre {
 
-struct AttendParams {
+constexpr int kM = 128;        // q rows of a tile
+constexpr int kN = 128;        // key rows of a step
+constexpr int kThreads = 320;
+constexpr int kMmaWarp = 8, kLoadWarp = 9;
+constexpr uint32_t kTmemCols = 512;
+
+struct Params {
   rkv_gqa_view cache;
   int layer;
-  const uint16_t* q;
-  int64_t q_ts, q_hs;
-  int64_t n_tokens;
-  int n_q_heads;
+  int n_tokens, n_q_heads, group, tile_tokens;  // tokens of a tile: 128 / group
   const int32_t* cu_q;
   int n_seq;
   const int32_t* page_table;
@@ -26,111 +51,602 @@ struct AttendParams {
   int window;
   const float* sinks;
   float scale_log2;
+  int n_splits;
+  float* part_o;   // [n_splits][n_tokens][n_q_heads][head_dim]
+  float* part_ml;  // [n_splits][n_tokens][n_q_heads][2]
   uint16_t* out;
   uint32_t* status;
 };
 
-template <typename T, int D>
-__global__ void __launch_bounds__(128) attend_kernel(const AttendParams p) {
-  constexpr int kWords = D / 64;  // words of two lanes each
-  const int lane = threadIdx.x & 31;
-  const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  const int64_t t = item / p.n_q_heads;
-  const int h = (int)(item % p.n_q_heads);
-  if (t >= p.n_tokens) return;
-  int seq = 0, hi = p.n_seq;  // the last sequence that starts at or before t
-  while (hi - seq > 1) {
-    const int mid = (seq + hi) / 2;
-    if (p.cu_q[mid] <= t) seq = mid;
-    else hi = mid;
-  }
-  if (t < p.cu_q[seq] || t >= p.cu_q[seq + 1]) {
-    if (lane == 0) set_status(p.status, RKV_ERR_INDEX_OUT_OF_RANGE);
-    return;
-  }
-  const int q_len = p.cu_q[seq + 1] - p.cu_q[seq];
-  const int i = (int)(t - p.cu_q[seq]);
-  int64_t len = p.kv_lens[seq];
-  if (len < 0 || len > p.pt_stride * kPage) {
-    if (lane == 0) set_status(p.status, RKV_ERR_INDEX_OUT_OF_RANGE);
-    len = len < 0 ? 0 : p.pt_stride * kPage;
-  }
-  const int64_t at = len - q_len + i;
-  const int64_t first = p.window > 0 && at >= p.window ? at - p.window + 1 : 0;
-  const int hkv = h / (p.n_q_heads / p.cache.n_kv_heads);
-  const uint16_t* qp = p.q + t * p.q_ts + h * p.q_hs + lane * 2 * kWords;
-  float2 q[kWords], acc[kWords];
-#pragma unroll
-  for (int w = 0; w < kWords; ++w) {
-    q[w] = T::unpack(reinterpret_cast<const uint32_t*>(qp)[w]);
-    acc[w] = make_float2(0.f, 0.f);
-  }
-  float m = p.sinks ? p.sinks[h] * 1.4426950408889634f : -INFINITY, l = p.sinks ? 1.0f : 0.0f;
-  for (int64_t j = first; j <= at; ++j) {
-    const int32_t page = p.page_table[seq * p.pt_stride + j / kPage];
-    uint32_t k[kWords], v[kWords];
-    if (page >= 0 && page < p.cache.n_pages) {
-      const uint16_t* base = static_cast<const uint16_t*>(p.cache.base) + lane * 2 * kWords;
-      const uint32_t* kp = reinterpret_cast<const uint32_t*>(base + (row_base(p.cache, p.layer, page, 0, hkv) + j % kPage) * D);
-      const uint32_t* vp = reinterpret_cast<const uint32_t*>(base + (row_base(p.cache, p.layer, page, 1, hkv) + j % kPage) * D);
-#pragma unroll
-      for (int w = 0; w < kWords; ++w) k[w] = kp[w], v[w] = vp[w];
-    } else {
-      if (lane == 0) set_status(p.status, RKV_ERR_INDEX_OUT_OF_RANGE);
-#pragma unroll
-      for (int w = 0; w < kWords; ++w) k[w] = v[w] = 0u;
-    }
-    float x = 0.f;
-#pragma unroll
-    for (int w = 0; w < kWords; ++w) {
-      const float2 f = T::unpack(k[w]);
-      x += q[w].x * f.x + q[w].y * f.y;
-    }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-    x *= p.scale_log2;
-    const float top = fmaxf(m, x);
-    const float old = m == -INFINITY ? 0.f : ex2(m - top), e = ex2(x - top);
-    m = top;
-    l = l * old + e;
-#pragma unroll
-    for (int w = 0; w < kWords; ++w) {
-      const float2 f = T::unpack(v[w]);
-      acc[w] = make_float2(acc[w].x * old + e * f.x, acc[w].y * old + e * f.y);
-    }
-  }
-  const float inv = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);
-  uint32_t* op = reinterpret_cast<uint32_t*>(p.out + (t * p.n_q_heads + h) * D + lane * 2 * kWords);
-#pragma unroll
-  for (int w = 0; w < kWords; ++w) op[w] = T::pack(acc[w].x * inv, acc[w].y * inv);
+template <int D>
+struct Layout {
+  static constexpr int kQ = kM * D * 2;      // bytes of a Q tile
+  static constexpr int kStage = kN * D * 2;  // K or V of a step
+  static constexpr int kStages = D == 128 ? 5 : 8;
+  static constexpr int kCol = 128 * 128;     // a 64-lane column block of 128 rows
+  static constexpr int kRing = 2 * kQ;
+  static constexpr int kBars = kRing + kStages * kStage;
+  // full[kStages], empty[kStages], S full x 2, P full x 2, O full x 2, Q full, drain
+  static constexpr int kBarEmpty = 8 * kStages, kBarS = 16 * kStages, kBarP = kBarS + 16, kBarO = kBarP + 16,
+                       kBarQ = kBarO + 16, kBarDrain = kBarQ + 8;
+  static constexpr int kMisc = kBars + kBarDrain + 8;  // TMEM address, abort flag, scan, found
+  static constexpr int kTotal = kMisc + 128 + 1024;
+};
+
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ bool elect_one() {
+  uint32_t pred = 0;
+  asm volatile("{\n\t.reg .pred P;\n\telect.sync _|P, 0xffffffff;\n\tselp.u32 %0, 1, 0, P;\n\t}" : "=r"(pred));
+  return pred != 0;
+}
+__device__ __forceinline__ void mma_commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+// D = A B (+ D): A in shared memory, or (ta) in tensor memory.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+// 128-byte-swizzle matrix descriptor.
+__device__ __forceinline__ uint64_t sw128_desc(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
+  return (uint64_t)((saddr >> 4) & 0x3fffu) | ((uint64_t)((lbo >> 4) & 0x3fffu) << 16) |
+         ((uint64_t)((sbo >> 4) & 0x3fffu) << 32) | (1ull << 46) | (2ull << 61);
+}
+// A warp's 32 lanes x 32 columns: thread t holds lane t.
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
+      "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(addr));
+}
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"
+      "%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+      "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]),
+      "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]),
+      "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
+          addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+      "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+// max(a, b, c) in one instruction (sm_100); NaN handling as fmaxf.
+__device__ __forceinline__ float fmax3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ unsigned long long pk2(uint32_t lo, uint32_t hi) {
+  return ((unsigned long long)hi << 32) | lo;
+}
+__device__ __forceinline__ unsigned long long dup2(float x) { return pk2(__float_as_uint(x), __float_as_uint(x)); }
+
+// The new tokens of sequence s in q: [begin, end), cut to what q holds.
+__device__ __forceinline__ int2 new_tokens(const Params& p, int s) {
+  const int a = min(max(__ldg(p.cu_q + s), 0), p.n_tokens);
+  return make_int2(a, min(max(__ldg(p.cu_q + s + 1), a), p.n_tokens));
 }
 
-static rkv_status attend(const AttendParams& p, const char* what, cudaStream_t s) {
-  const int64_t blocks = (p.n_tokens * p.n_q_heads + 3) / 4;
-  if (blocks > INT32_MAX) return fail(RKV_ERR_SHAPE_MISMATCH, "%s: too many tokens", what);
-  if (p.cache.dtype == RKV_GQA_BF16) {
-    if (p.cache.head_dim == 64) attend_kernel<Bf16, 64><<<(unsigned)blocks, 128, 0, s>>>(p);
-    else attend_kernel<Bf16, 128><<<(unsigned)blocks, 128, 0, s>>>(p);
+// What a CTA works on, the same for all of its threads.
+struct Work {
+  int head;         // kv head
+  int seq;
+  int token;        // first token (row of q)
+  int tokens;       // tokens of both tiles
+  int pos;          // position of the first token, may be negative
+  int len;          // rows of the sequence
+  int step0, steps; // 128-row steps of this CTA's split
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, 1)
+prefill_kernel(const Params p, const __grid_constant__ CUtensorMap map, const __grid_constant__ CUtensorMap qmap) {
+  using L = Layout<D>;
+  extern __shared__ uint8_t raw[];
+  uint8_t* smem = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
+  const uint32_t base = smem_u32(smem), bars = base + L::kBars;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kMisc);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kMisc + 4);
+  int* scan = reinterpret_cast<int*>(smem + L::kMisc + 8);    // [12] per warp
+  int* found = reinterpret_cast<int*>(smem + L::kMisc + 64);  // sequence, block within it
+
+  if (tid == 0) {
+    for (int i = 0; i < L::kStages; ++i) {
+      mbar_init(bars + 8 * i, 1);
+      mbar_init(bars + L::kBarEmpty + 8 * i, 1);
+    }
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(bars + L::kBarS + 8 * t, 1);
+      mbar_init(bars + L::kBarP + 8 * t, 128);
+      mbar_init(bars + L::kBarO + 8 * t, 1);
+    }
+    mbar_init(bars + L::kBarQ, 1);
+    mbar_init(bars + L::kBarDrain, 1);
+    *abort_flag = 0;
+    found[0] = -1;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&map) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&qmap) : "memory");
+  }
+  if (warp == kMmaWarp) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                 "r"(kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  // q rows that no token has (groups that do not divide 128): zeros
+  const int used = p.tile_tokens * p.group;
+  for (int i = tid; i < 2 * (kM - used) * (D / 8); i += kThreads) {
+    const int chunk = i % (D / 8), r = used + (i / (D / 8)) % (kM - used), t = i / ((D / 8) * (kM - used));
+    *reinterpret_cast<uint4*>(smem + t * L::kQ + (chunk >> 3) * L::kCol + r * 128 + (((chunk & 7) ^ (r & 7)) << 4)) =
+        make_uint4(0, 0, 0, 0);
+  }
+  fence_proxy_async();
+  grid_dependency_wait();
+  grid_launch_dependents();
+
+  // ---- which sequence and tokens: blocks of two tiles, the last tokens first
+  const int span = 2 * p.tile_tokens;
+  const int rank = blockIdx.x / p.cache.n_kv_heads;
+  {
+    const int per = (p.n_seq + kThreads - 1) / kThreads;
+    const int s_begin = min(tid * per, p.n_seq), s_end = min(s_begin + per, p.n_seq);
+    int mine = 0;
+    for (int s = s_begin; s < s_end; ++s) {
+      const int2 t = new_tokens(p, s);
+      mine += (t.y - t.x + span - 1) / span;
+    }
+    int upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += v;
+    }
+    if (lane == 31) scan[warp] = upto;
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    for (int w = 0; w < warp; ++w) upto += scan[w];
+    int at = upto - mine;
+    if (rank >= at && rank < upto) {
+      for (int s = s_begin; s < s_end; ++s) {
+        const int2 t = new_tokens(p, s);
+        const int n = (t.y - t.x + span - 1) / span;
+        if (rank < at + n) {
+          found[0] = s;
+          found[1] = n - 1 - (rank - at);
+          break;
+        }
+        at += n;
+      }
+    }
+    __syncthreads();
+  }
+  const uint32_t tmem = *tmem_slot;
+  Work w;
+  w.seq = found[0];
+  w.steps = 0;
+  if (w.seq >= 0) {
+    const int2 t = new_tokens(p, w.seq);
+    w.head = blockIdx.x % p.cache.n_kv_heads;
+    const int first = found[1] * span;
+    w.token = t.x + first;
+    w.tokens = min(span, t.y - t.x - first);
+    const int given = __ldg(p.kv_lens + w.seq), most = (int)p.pt_stride * kPage;
+    w.len = min(max(given, 0), most);
+    w.pos = w.len - (t.y - t.x) + first;
+    const int end = w.pos + w.tokens;  // rows [.., end) are seen
+    const int begin = p.window > 0 ? max(0, w.pos - p.window + 1) : 0;
+    const int s0 = begin / kN, s1 = end > 0 ? (end + kN - 1) / kN : 0;
+    const int per = (max(0, s1 - s0) + p.n_splits - 1) / p.n_splits;
+    w.step0 = s0 + blockIdx.y * per;
+    w.steps = max(0, min(per, s1 - w.step0));
+    if (tid == 0 && (given != w.len || __ldg(p.cu_q) != 0 || __ldg(p.cu_q + p.n_seq) != p.n_tokens ||
+                     t.x != __ldg(p.cu_q + w.seq) || t.y != __ldg(p.cu_q + w.seq + 1)))
+      set_status(p.status, RKV_ERR_INDEX_OUT_OF_RANGE);
+  }
+  const int tiles = w.tokens > p.tile_tokens ? 2 : 1;
+
+  if (warp >= kMmaWarp) {
+    if (warp == kMmaWarp && w.steps > 0) {
+      // ------------------------------------------------------------ MMA issuer
+      constexpr uint32_t kType = T::kCode == RKV_GQA_BF16 ? (1u << 7) | (1u << 10) : 0u;
+      constexpr uint32_t kIdescS = (1u << 4) | kType | ((kN >> 3) << 17) | ((kM >> 4) << 24);
+      constexpr uint32_t kIdescO = (1u << 4) | kType | (1u << 16) | ((D >> 3) << 17) | ((kM >> 4) << 24);
+      bool ok = __all_sync(0xffffffffu, mbar_wait(bars + L::kBarQ, 0, abort_flag));
+      // O_t += P_t V of step j
+      auto pv = [&](int t, int j) {
+        const uint32_t vs = base + L::kRing + ((2 * j + 1) % L::kStages) * L::kStage;
+        const uint64_t vd = sw128_desc(vs, L::kCol, 1024);
+        const uint32_t o = tmem + 256 + t * D, pa = tmem + t * 128;
+#pragma unroll
+        for (int k = 0; k < kN / 16; ++k)
+          mma_ts(o, pa + 8 * k, vd + (uint64_t)((k * 2048) >> 4), kIdescO, (j > 0 || k > 0) ? 1u : 0u);
+      };
+      // waits for V of step j and clears what lies past the sequence's end in it
+      auto v_ready = [&](int j) {
+        const int st = (2 * j + 1) % L::kStages;
+        if (!__all_sync(0xffffffffu, mbar_wait(bars + 8 * st, ((2 * j + 1) / L::kStages) & 1, abort_flag))) return false;
+        const int past = w.len - (w.step0 + j) * kN;  // first row past the end
+        if (past < kN && past % kPage != 0) {
+          const int stop = (past + kPage - 1) / kPage * kPage;
+          for (int i = lane; i < (stop - past) * (D / 8); i += 32) {
+            const int r = past + i / (D / 8), c = i % (D / 8);
+            *reinterpret_cast<uint4*>(smem + L::kRing + st * L::kStage + (c >> 3) * L::kCol + r * 128 +
+                                      (((c & 7) ^ (r & 7)) << 4)) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async();
+          __syncwarp();
+        }
+        return true;
+      };
+      for (int j = 0; ok && j < w.steps; ++j) {
+        const int st = (2 * j) % L::kStages;
+        ok = __all_sync(0xffffffffu, mbar_wait(bars + 8 * st, ((2 * j) / L::kStages) & 1, abort_flag));
+        if (ok && j > 0) ok = v_ready(j - 1);
+        for (int t = 0; ok && t < tiles; ++t) {
+          if (j > 0) ok = __all_sync(0xffffffffu, mbar_wait(bars + L::kBarP + 8 * t, (j - 1) & 1, abort_flag));
+          if (!ok) break;
+          tc_fence_after();
+          if (elect_one()) {
+            if (j > 0) {
+              pv(t, j - 1);
+              if (t == tiles - 1) mma_commit(bars + L::kBarEmpty + 8 * ((2 * j - 1) % L::kStages));
+            }
+            const uint64_t qd = sw128_desc(base + t * L::kQ, 16, 1024);
+            const uint64_t kd = sw128_desc(base + L::kRing + st * L::kStage, 16, 1024);
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k) {
+              const uint64_t off = (uint64_t)(((k >> 2) * L::kCol + (k & 3) * 32) >> 4);
+              mma_ss(tmem + t * 128, qd + off, kd + off, kIdescS, k > 0);
+            }
+            mma_commit(bars + L::kBarS + 8 * t);
+            if (t == tiles - 1) mma_commit(bars + L::kBarEmpty + 8 * st);
+          }
+          __syncwarp();
+        }
+      }
+      if (ok) ok = v_ready(w.steps - 1);
+      for (int t = 0; ok && t < tiles; ++t) {
+        ok = __all_sync(0xffffffffu, mbar_wait(bars + L::kBarP + 8 * t, (w.steps - 1) & 1, abort_flag));
+        if (!ok) break;
+        tc_fence_after();
+        if (elect_one()) {
+          pv(t, w.steps - 1);
+          mma_commit(bars + L::kBarO + 8 * t);
+        }
+        __syncwarp();
+      }
+      if (!ok) {
+        *abort_flag = 1;
+        set_status(p.status, RKV_ERR_CUDA);
+      }
+      // every MMA is done before the tensor memory is freed
+      if (elect_one()) mma_commit(bars + L::kBarDrain);
+      __syncwarp();
+      mbar_wait_copy(bars + L::kBarDrain, 0);
+    } else if (warp == kLoadWarp && w.steps > 0) {
+      // ---------------------------------------------------------------- loader
+      const int rows_total = (int)row_base(p.cache, p.cache.n_layers, 0, 0, 0);  // out of range: zero rows
+      const int v_off = p.cache.n_kv_heads * kPage;
+      if (lane == 0) {
+        mbar_expect_tx(bars + L::kBarQ, tiles * (D / 64) * used * 128);
+        for (int t = 0; t < tiles; ++t)
+          for (int c = 0; c < D / 64; ++c)
+            asm volatile(
+                "cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, "
+                "%4}], [%5];" ::"r"(base + t * L::kQ + c * L::kCol),
+                "l"(&qmap), "r"(64 * c), "r"(w.head * p.group), "r"(w.token + t * p.tile_tokens), "r"(bars + L::kBarQ)
+                : "memory");
+      }
+      const int32_t* ids = p.page_table + w.seq * p.pt_stride;
+      const int page_end = (w.len + kPage - 1) / kPage;
+      bool ok = true;
+      int n = 0;  // stages filled
+      for (int at = 0; at < 2 * w.steps && ok; at += 32) {
+        const int pg = 2 * w.step0 + at + lane;
+        int row = rows_total;
+        if (at + lane < 2 * w.steps && pg < page_end) {
+          const int id = __ldg(ids + pg);
+          if (id >= 0 && id < p.cache.n_pages) row = (int)row_base(p.cache, p.layer, id, 0, w.head);
+          else set_status(p.status, RKV_ERR_INDEX_OUT_OF_RANGE);
+        }
+        for (int i = 0; i < 32 && at + i < 2 * w.steps && ok; i += 2) {
+          const int y0 = __shfl_sync(0xffffffffu, row, i), y1 = __shfl_sync(0xffffffffu, row, i + 1);
+          for (int kv = 0; kv < 2; ++kv, ++n) {
+            const int st = n % L::kStages;
+            if (n >= L::kStages &&
+                !__all_sync(0xffffffffu, mbar_wait(bars + L::kBarEmpty + 8 * st, (n / L::kStages - 1) & 1, abort_flag))) {
+              ok = false;
+              break;
+            }
+            if (lane == 0) {
+              const uint32_t full = bars + 8 * st, dst = base + L::kRing + st * L::kStage;
+              mbar_expect_tx(full, L::kStage);
+#pragma unroll
+              for (int c = 0; c < D / 64; ++c) {
+                tma_load_2d(dst + c * L::kCol, &map, 64 * c, y0 == rows_total ? y0 : y0 + kv * v_off, full);
+                tma_load_2d(dst + c * L::kCol + 8192, &map, 64 * c, y1 == rows_total ? y1 : y1 + kv * v_off, full);
+              }
+            }
+          }
+        }
+      }
+      if (!ok) {
+        *abort_flag = 1;
+        set_status(p.status, RKV_ERR_CUDA);
+      }
+      // every copy has landed before the CTA ends
+      mbar_wait_copy(bars + L::kBarQ, 0);
+      for (int i = max(0, n - L::kStages); i < n; ++i)
+        mbar_wait_copy(bars + 8 * (i % L::kStages), (i / L::kStages) & 1);
+    }
   } else {
-    if (p.cache.head_dim == 64) attend_kernel<F16, 64><<<(unsigned)blocks, 128, 0, s>>>(p);
-    else attend_kernel<F16, 128><<<(unsigned)blocks, 128, 0, s>>>(p);
+    // --------------------------------------------------------------- softmax
+    const int t = warp >> 2;                           // tile
+    const int r = 32 * (warp & 3) + lane;              // row of the tile
+    const int token = t * p.tile_tokens + r / p.group; // of the CTA's tokens
+    const bool live = w.seq >= 0 && r < used && token < w.tokens;
+    const uint32_t ts = tmem + t * 128 + ((uint32_t)(32 * (warp & 3)) << 16);
+    const uint32_t to = ts - t * 128 + 256 + t * D;
+    const int pos = w.pos + token;  // this row's position
+    const int pos_min = w.pos + t * p.tile_tokens;  // the tile's first and last
+    const int pos_max = pos_min + p.tile_tokens - 1;
+    float m = -INFINITY;                 // exponent reference
+    float l = 0.f;
+    bool ok = true;
+    if (w.seq >= 0 && t < tiles && w.steps > 0) {
+      const unsigned long long c2 = dup2(p.scale_log2);
+      for (int j = 0; j < w.steps; ++j) {
+        if (!__all_sync(0xffffffffu, mbar_wait(bars + L::kBarS + 8 * t, j & 1, abort_flag))) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        uint32_t x[kN];
+#pragma unroll
+        for (int i = 0; i < kN; i += 32) tmem_ld32(ts + i, x + i);
+        tmem_wait_ld();
+        const int key0 = (w.step0 + j) * kN;
+        if (key0 + kN - 1 > pos_min || (p.window > 0 && key0 <= pos_max - p.window)) {
+          const int last = pos - key0, first = p.window > 0 ? last - p.window : -1;
+#pragma unroll
+          for (int i = 0; i < kN; ++i)
+            if (i > last || i <= first) x[i] = 0xff800000u;  // -inf
+        }
+        float t0 = __uint_as_float(x[0]), t1 = __uint_as_float(x[1]), t2 = __uint_as_float(x[2]),
+              t3 = __uint_as_float(x[3]);
+#pragma unroll
+        for (int i = 4; i < kN - 4; i += 8) {
+          t0 = fmax3(t0, __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
+          t1 = fmax3(t1, __uint_as_float(x[i + 2]), __uint_as_float(x[i + 3]));
+          t2 = fmax3(t2, __uint_as_float(x[i + 4]), __uint_as_float(x[i + 5]));
+          t3 = fmax3(t3, __uint_as_float(x[i + 6]), __uint_as_float(x[i + 7]));
+        }
+        t0 = fmax3(t0, __uint_as_float(x[kN - 4]), __uint_as_float(x[kN - 3]));
+        t1 = fmax3(t1, __uint_as_float(x[kN - 2]), __uint_as_float(x[kN - 1]));
+        const float top = fmaxf(fmax3(t0, t1, t2), t3) * p.scale_log2 - SoftmaxBias<T>::kBias;
+        const bool up = top > m + kLazyLog2 || (m == -INFINITY && top > -INFINITY);
+        if (__any_sync(0xffffffffu, up)) {
+          const float a = up ? ex2(m - top) : 1.f;  // 0 from -inf
+          m = up ? top : m;
+          l *= a;
+          if (j > 0) {  // the MMAs of the step before are done: S was committed after them
+#pragma unroll 1
+            for (int c = 0; c < D; c += 32) {
+              uint32_t o[32];
+              tmem_ld32(to + c, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * a);
+              tmem_st32(to + c, o);
+            }
+          }
+        }
+        const unsigned long long n2 = dup2(m == -INFINITY ? 0.f : -m);  // nothing seen yet: weights 0
+        unsigned long long sum0 = 0ull, sum1 = 0ull;
+#pragma unroll
+        for (int i = 0; i < kN; i += 32) {
+          uint32_t pw[16];
+#pragma unroll
+          for (int k = 0; k < 32; k += 4) {
+            const unsigned long long a2 = fma_f32x2(pk2(x[i + k], x[i + k + 1]), c2, n2);
+            const unsigned long long b2 = fma_f32x2(pk2(x[i + k + 2], x[i + k + 3]), c2, n2);
+            const float e0 = ex2(__uint_as_float((uint32_t)a2)), e1 = ex2(__uint_as_float((uint32_t)(a2 >> 32)));
+            const float e2 = ex2(__uint_as_float((uint32_t)b2)), e3 = ex2(__uint_as_float((uint32_t)(b2 >> 32)));
+            sum0 = add_f32x2(sum0, pk2(__float_as_uint(e0), __float_as_uint(e1)));
+            sum1 = add_f32x2(sum1, pk2(__float_as_uint(e2), __float_as_uint(e3)));
+            pw[k / 2] = T::pack(e0, e1);
+            pw[k / 2 + 1] = T::pack(e2, e3);
+          }
+          tmem_st16(ts + i / 2, pw);
+        }
+        const unsigned long long sum = add_f32x2(sum0, sum1);
+        l += __uint_as_float((uint32_t)sum) + __uint_as_float((uint32_t)(sum >> 32));
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(bars + L::kBarP + 8 * t);
+      }
+      if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bars + L::kBarO + 8 * t, 0, abort_flag));
+      if (!ok) {
+        *abort_flag = 1;
+        set_status(p.status, RKV_ERR_CUDA);
+      }
+      tc_fence_after();
+    }
+    // ---- epilogue: one row a thread
+    if (w.seq >= 0 && t < tiles) {
+      const int head = w.head * p.group + r % p.group;
+      const int64_t row = (int64_t)(w.token + token) * p.n_q_heads + head;
+      const bool have = ok && w.steps > 0;
+      float f = 1.f;
+      float* part = nullptr;
+      if (p.n_splits > 1) {
+        const int64_t at = (int64_t)blockIdx.y * p.n_tokens * p.n_q_heads + row;
+        part = p.part_o + at * D;
+        if (live) *reinterpret_cast<float2*>(p.part_ml + 2 * at) = make_float2(have ? m : -INFINITY, l);
+      } else if (live) {
+        const float sink = p.sinks ? p.sinks[head] * 1.4426950408889634f : -INFINITY;
+        const float top = fmaxf(m, sink);
+        const float e = ex2(m - top);
+        f = m == -INFINITY ? 0.f : e / (l * e + ex2(sink - top));
+      }
+#pragma unroll 1
+      for (int c = 0; c < D; c += 32) {
+        uint32_t o[32];
+        if (have) {
+          tmem_ld32(to + c, o);
+          tmem_wait_ld();
+        }
+        if (!live) continue;
+        const bool seen = have && m != -INFINITY;  // a row that saw nothing: zeros, whatever O holds
+#pragma unroll
+        for (int i = 0; i < 32; ++i) o[i] = seen ? __float_as_uint(__uint_as_float(o[i]) * f) : 0u;
+        if (part) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 4)
+            *reinterpret_cast<uint4*>(part + c + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; i += 8) {
+            uint4 v;
+            v.x = T::pack(__uint_as_float(o[i]), __uint_as_float(o[i + 1]));
+            v.y = T::pack(__uint_as_float(o[i + 2]), __uint_as_float(o[i + 3]));
+            v.z = T::pack(__uint_as_float(o[i + 4]), __uint_as_float(o[i + 5]));
+            v.w = T::pack(__uint_as_float(o[i + 6]), __uint_as_float(o[i + 7]));
+            *reinterpret_cast<uint4*>(p.out + row * D + c + i) = v;
+          }
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == kMmaWarp)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+}
+
+// Joins the splits of one (token, q head) a warp, in their order.
+template <typename T, int D>
+__global__ void __launch_bounds__(128) join_kernel(const Params p) {
+  grid_dependency_wait();
+  const int64_t rows = (int64_t)p.n_tokens * p.n_q_heads;
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (row >= rows) return;
+  const int lane = threadIdx.x & 31;
+  const int head = (int)(row % p.n_q_heads);
+  const float sink = p.sinks ? p.sinks[head] * 1.4426950408889634f : -INFINITY;
+  float top = sink;
+  for (int i = 0; i < p.n_splits; ++i) top = fmaxf(top, p.part_ml[2 * (i * rows + row)]);
+  if (top == -INFINITY) top = 0.f;
+  float o[D / 32] = {};
+  float l = ex2(sink - top);
+  for (int i = 0; i < p.n_splits; ++i) {
+    const int64_t at = i * rows + row;
+    const float2 e = *reinterpret_cast<const float2*>(p.part_ml + 2 * at);
+    if (e.x == -INFINITY) continue;
+    const float w = ex2(e.x - top);
+    l += w * e.y;
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j) o[j] += w * p.part_o[at * D + D / 32 * lane + j];
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+  for (int j = 0; j < D / 32; j += 2)
+    *reinterpret_cast<uint32_t*>(p.out + row * D + D / 32 * lane + j) = T::pack(o[j] * inv, o[j + 1] * inv);
+}
+
+template <typename T, int D>
+static rkv_status launch(const Params& p, const CUtensorMap& map, const CUtensorMap& qmap, cudaStream_t s,
+                         const char* what) {
+  static std::atomic<bool> ready[kMaxDevicesCached];  // the shared-memory opt-in is per device
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= kMaxDevicesCached || !ready[dev].load(std::memory_order_acquire)) {
+    const cudaError_t e =
+        cudaFuncSetAttribute(prefill_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<D>::kTotal);
+    if (e != cudaSuccess) return fail(RKV_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
+    if (dev >= 0 && dev < kMaxDevicesCached) ready[dev].store(true, std::memory_order_release);
+  }
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  // every sequence rounds its tokens up to whole blocks: at most one more each
+  const int64_t blocks = ((int64_t)p.n_tokens / (2 * p.tile_tokens) + p.n_seq) * p.cache.n_kv_heads;
+  if (blocks > INT32_MAX) return fail(RKV_ERR_SHAPE_MISMATCH, "%s: too many tokens", what);
+  cfg.gridDim = dim3((unsigned)blocks, (unsigned)p.n_splits);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = Layout<D>::kTotal;
+  cfg.stream = s;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, prefill_kernel<T, D>, p, map, qmap);
+  if (e == cudaSuccess && p.n_splits > 1) {
+    cfg.gridDim = dim3((unsigned)(((int64_t)p.n_tokens * p.n_q_heads + 3) / 4));
+    cfg.blockDim = dim3(128);
+    cfg.dynamicSmemBytes = 0;
+    e = cudaLaunchKernelEx(&cfg, join_kernel<T, D>, p);
+  }
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return fail(RKV_ERR_CUDA, "%s: launch failed: %s", what, cudaGetErrorString(e));
   }
   return check_launch(what);
 }
 
+}  // namespace pre
 }  // namespace gqa
 }  // namespace rkv
 
 extern "C" int32_t rkv_gqa_prefill_splits(const rkv_gqa_view* cache, int64_t n_tokens, int32_t n_q_heads,
                                           int32_t n_seq, int64_t pt_stride) {
-  if (!cache || n_tokens < 0 || n_q_heads < 1 || n_seq < 0 || pt_stride < 1) return -1;
-  return 1;
+  if (!cache || n_tokens < 0 || n_q_heads < 1 || n_seq < 0 || pt_stride < 1 || cache->n_kv_heads < 1 ||
+      n_q_heads % cache->n_kv_heads != 0 || n_q_heads / cache->n_kv_heads > RKV_GQA_MAX_GROUP)
+    return -1;
+  // CTAs of the tokens alone; with fewer than half the SMs busy, cut the rows so that the SMs are covered, but
+  // not below 8 steps of 128 rows
+  const int64_t span = 2 * (128 / (n_q_heads / cache->n_kv_heads));
+  int64_t blocks = (n_tokens + span - 1) / span;
+  if (blocks < n_seq) blocks = n_seq;
+  blocks *= cache->n_kv_heads;
+  if (blocks == 0 || 2 * blocks > 148) return 1;
+  int64_t splits = 148 / blocks;
+  const int64_t most = pt_stride / 16;
+  if (splits > most) splits = most;
+  return splits < 1 ? 1 : splits > 64 ? 64 : (int32_t)splits;
 }
 
 extern "C" int64_t rkv_gqa_prefill_workspace_bytes(const rkv_gqa_view* cache, int64_t n_tokens, int32_t n_q_heads,
                                                    int32_t n_splits) {
   if (!cache || n_tokens < 0 || n_q_heads < 1 || n_splits < 1) return -1;
-  return 0;
+  return n_splits == 1 ? 0 : n_splits * n_tokens * n_q_heads * (cache->head_dim + 2) * 4;
 }
 
 extern "C" rkv_status rkv_gqa_prefill(const rkv_gqa_view* cache, int32_t layer, const void* q, int64_t q_token_stride,
@@ -141,11 +657,12 @@ extern "C" rkv_status rkv_gqa_prefill(const rkv_gqa_view* cache, int32_t layer, 
                                       rkv_stream_t stream) {
   using namespace rkv;
   using namespace rkv::gqa;
+  using namespace rkv::gqa::pre;
   static const char* what = "rkv_gqa_prefill";
   rkv_status st = check_cache(cache, layer, what);
   if (st != RKV_OK) return st;
   if ((st = check_heads(cache, n_q_heads, what)) != RKV_OK) return st;
-  if (n_tokens < 0 || n_tokens > INT32_MAX) return fail_shape("n_tokens", 0, n_tokens, "%s: bad n_tokens", what);
+  if (n_tokens < 0 || n_tokens > INT32_MAX / 2) return fail_shape("n_tokens", 0, n_tokens, "%s: bad n_tokens", what);
   if (n_seq < 0) return fail_shape("n_seq", 0, n_seq, "%s: n_seq < 0", what);
   if (n_splits < 1 || n_splits > 64) return fail_shape("n_splits", 1, n_splits, "%s: 1 <= n_splits <= 64", what);
   if (n_tokens == 0 || n_seq == 0) {
@@ -155,14 +672,36 @@ extern "C" rkv_status rkv_gqa_prefill(const rkv_gqa_view* cache, int32_t layer, 
   }
   const AttendArgs args = {*cache,     layer,   q,      q_token_stride, q_head_stride, n_tokens, n_q_heads, page_table,
                            pt_stride,  kv_lens, window, sinks,          softmax_scale, out,      d_status};
-  st = check_attend(args, what);
-  if (st != RKV_OK) return st;
+  if ((st = check_attend(args, what)) != RKV_OK) return st;
   if (!cu_q) return fail(RKV_ERR_INVALID_ARGUMENT, "%s: cu_q is required", what);
-  const AttendParams p = {*cache,    layer,      static_cast<const uint16_t*>(q),
-                          q_token_stride, q_head_stride, n_tokens,
-                          n_q_heads, cu_q,       n_seq,
-                          page_table, pt_stride, kv_lens,
-                          window,    sinks,      (float)((double)softmax_scale * 1.4426950408889634),
-                          static_cast<uint16_t*>(out), d_status};
-  return attend(p, what, (cudaStream_t)stream);
+  if (n_splits > 1 && (!workspace || !aligned(workspace, 16)))
+    return fail(RKV_ERR_INVALID_ARGUMENT, "%s: a 16-byte aligned workspace is required", what);
+  Params p;
+  p.cache = *cache;
+  p.layer = layer;
+  p.n_tokens = (int)n_tokens;
+  p.n_q_heads = n_q_heads;
+  p.group = n_q_heads / cache->n_kv_heads;
+  p.tile_tokens = kM / p.group;
+  p.cu_q = cu_q;
+  p.n_seq = n_seq;
+  p.page_table = page_table;
+  p.pt_stride = pt_stride;
+  p.kv_lens = kv_lens;
+  p.window = window;
+  p.sinks = sinks;
+  p.scale_log2 = (float)((double)softmax_scale * 1.4426950408889634);
+  p.n_splits = n_splits;
+  p.part_o = static_cast<float*>(workspace);
+  p.part_ml = workspace ? p.part_o + n_splits * n_tokens * n_q_heads * cache->head_dim : nullptr;
+  p.out = static_cast<uint16_t*>(out);
+  p.status = d_status;
+  CUtensorMap map, qmap;
+  if ((st = cache_map(*cache, &map, what)) != RKV_OK) return st;
+  if ((st = q_map(*cache, q, q_token_stride, q_head_stride, n_tokens, n_q_heads, p.tile_tokens, p.group, &qmap, what)) != RKV_OK)
+    return st;
+  cudaStream_t s = (cudaStream_t)stream;
+  if (cache->dtype == RKV_GQA_BF16)
+    return cache->head_dim == 64 ? launch<Bf16, 64>(p, map, qmap, s, what) : launch<Bf16, 128>(p, map, qmap, s, what);
+  return cache->head_dim == 64 ? launch<F16, 64>(p, map, qmap, s, what) : launch<F16, 128>(p, map, qmap, s, what);
 }

@@ -128,7 +128,9 @@ class GqaKvPool:
             raise ShapeMismatch(f"{name}: expected [tokens, {heads or 'heads'}, {self.head_dim}], got {tuple(shape)}")
         if stride[2] != 1:
             raise ShapeMismatch(f"{name}: the {self.head_dim} elements of a row must be contiguous")
-        return t.data_ptr(), stride[0], stride[1]
+        # a stride that no second row uses may be anything
+        return (t.data_ptr(), stride[0] if shape[0] > 1 else shape[1] * shape[2],
+                stride[1] if shape[1] > 1 else shape[2])
 
     def _need(self, t: torch.Tensor, dtype: torch.dtype, name: str, shape: tuple) -> int:
         if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.device != self.device:
