@@ -82,7 +82,7 @@ __device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
 constexpr uint64_t kWaitNs = 1000000000ull;
 // Bounded wait (1 s) for the phase of the given parity; false on a timeout, or
 // as soon as another thread of the CTA gave up.
-static __device__ __noinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+__device__ __forceinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
   const uint64_t t0 = now_ns();
   while (!mbar_test(bar, parity)) {
     if (*abort_flag) return false;
@@ -96,7 +96,7 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
 }
 // The same for copies in flight: it ignores the abort flag, so that a CTA
 // never ends while one still writes into its shared memory.
-static __device__ __noinline__ bool mbar_wait_copy(uint32_t bar, uint32_t parity) {
+__device__ __forceinline__ bool mbar_wait_copy(uint32_t bar, uint32_t parity) {
   const uint64_t t0 = now_ns();
   while (!mbar_test(bar, parity))
     if (now_ns() - t0 > kWaitNs) return false;
