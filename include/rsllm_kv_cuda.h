@@ -741,32 +741,27 @@ RKV_API rkv_status rkv_gqa_copy_pages(const rkv_gqa_view* cache, const int32_t* 
  * its i-th new token sits at position p = kv_lens[s] - q_len + i and sees the
  * rows j <= p, with window > 0 only those with j > p - window.
  * out[t][h] = sum_j softmax_j(q . k_j * softmax_scale) v_j, in the cache's
- * type (contiguous [n_tokens][n_q_heads][head_dim], 16-byte aligned); sinks
+ * type (contiguous [n_tokens][n_q_heads][head_dim], 32-byte aligned); sinks
  * (f32 [n_q_heads] or NULL) add exp(sink) to a head's denominator.  A token that
  * sees no row gives zeros.
  * softmax_scale must be finite and > 0.
  * Device status: a page id outside the pool sets INDEX_OUT_OF_RANGE and reads
  * as zero rows; a length or offset outside the tables sets it too and is cut to
  * what they hold.
- * n_splits: each token's rows are cut into n_splits ranges that are processed in
- * parallel and joined through workspace (rkv_gqa_prefill_workspace_bytes bytes of
- * device memory, 16-byte aligned; may be NULL when n_splits == 1): for few new
- * tokens behind a long cached prefix.  rkv_gqa_prefill_splits says how many fill
- * the GPU (1 where the tokens alone do).
+ * The work is divided evenly over the GPU whatever the lengths; tokens whose rows
+ * are shared out are joined through workspace (rkv_gqa_prefill_workspace_bytes
+ * bytes of device memory, 32-byte aligned; its contents need no initialisation
+ * and do not outlast the call).
  * Numerics: logits and sums are f32; the weights are rounded to the cache's type
  * before their product with V, as the tensor cores take them.  A K or V row that
  * is not finite (rkv_gqa_append stores none) makes the tokens that see it NaN
  * and may do so to earlier tokens of its sequence. */
-RKV_API int32_t rkv_gqa_prefill_splits(const rkv_gqa_view* cache, int64_t n_tokens, int32_t n_q_heads, int32_t n_seq,
-                                       int64_t pt_stride);
-RKV_API int64_t rkv_gqa_prefill_workspace_bytes(const rkv_gqa_view* cache, int64_t n_tokens, int32_t n_q_heads,
-                                                int32_t n_splits);
+RKV_API int64_t rkv_gqa_prefill_workspace_bytes(const rkv_gqa_view* cache);
 RKV_API rkv_status rkv_gqa_prefill(const rkv_gqa_view* cache, int32_t layer, const void* q, int64_t q_token_stride,
                                    int64_t q_head_stride, int64_t n_tokens, int32_t n_q_heads, const int32_t* cu_q,
                                    int32_t n_seq, const int32_t* page_table, int64_t pt_stride,
                                    const int32_t* kv_lens, int32_t window, const float* sinks, float softmax_scale,
-                                   int32_t n_splits, void* workspace, void* out, uint32_t* d_status,
-                                   rkv_stream_t stream);
+                                   void* workspace, void* out, uint32_t* d_status, rkv_stream_t stream);
 
 /* Attention of one new token per sequence over the cache: rkv_gqa_prefill with
  * one token in each sequence (q and out [n_seq][n_q_heads][head_dim], the token

@@ -154,11 +154,9 @@ SIGNATURES = {
                                  _i32p, c_void_p, _i32p, c_void_p, c_int64, c_int64, c_int32, c_void_p, _u32p,
                                  c_void_p]),
     "rkv_gqa_copy_pages": (c_int32, [c_void_p, _i32p, _i32p, c_int64, _u32p, c_void_p]),
-    "rkv_gqa_prefill_splits": (c_int32, [c_void_p, c_int64, c_int32, c_int32, c_int64]),
-    "rkv_gqa_prefill_workspace_bytes": (c_int64, [c_void_p, c_int64, c_int32, c_int32]),
+    "rkv_gqa_prefill_workspace_bytes": (c_int64, [c_void_p]),
     "rkv_gqa_prefill": (c_int32, [c_void_p, c_int32, c_void_p, c_int64, c_int64, c_int64, c_int32, _i32p, c_int32,
-                                  _i32p, c_int64, _i32p, c_int32, _f32p, c_float, c_int32, c_void_p, c_void_p, _u32p,
-                                  c_void_p]),
+                                  _i32p, c_int64, _i32p, c_int32, _f32p, c_float, c_void_p, c_void_p, _u32p, c_void_p]),
     "rkv_gqa_decode_workspace_bytes": (c_int64, [c_void_p, c_int32, c_int32]),
     "rkv_gqa_decode": (c_int32, [c_void_p, c_int32, c_void_p, c_int64, c_int64, c_int32, c_int32, _i32p, c_int64,
                                  _i32p, c_int32, _f32p, c_float, c_void_p, c_void_p, _u32p, c_void_p]),

@@ -8,10 +8,19 @@
 // cores bound it, and close behind them the 16 exponentials a clock that an SM
 // evaluates (a 128 x 128 tile: 1024 clocks of each at head_dim 128).
 //
-// One CTA takes two tiles of 128 q rows of one kv head, against a page (64 key
-// rows) at a time.  A tile's rows are the group's q heads of 128 / group
+// A block is two tiles of 128 q rows of one kv head, taken against a page (64
+// key rows) at a time.  A tile's rows are the group's q heads of 128 / group
 // consecutive tokens, token by token, so that every K and V row fetched serves
 // the whole group and a tile of a long prompt has a short diagonal.
+//
+// One CTA runs on each SM.  The blocks of all sequences, in (sequence, head,
+// tokens) order and weighed by the rows they see, are cut into equal runs, one
+// for each CTA, so that ragged prompts, few tokens behind a long prefix and the
+// last wave of many leave no SM idle.  A run may begin and end inside a block
+// (not within 4 pages of its ends, nor in one of up to 8); such parts are
+// written as partial softmaxes (m, l, O) and joined by a second small kernel.
+// While a block ends, the next one's Q, K and V are copied and its first logits
+// computed.
 //
 //   warps 0-15      softmax, one row a thread: S from tensor memory, running
 //                   maximum and sum, P (in the cache's type) back over S; the
@@ -20,6 +29,7 @@
 //   warps 16, 17    issue S = Q K^T (Q, K in shared memory) and O += P V (P in
 //                   tensor memory, V in shared memory) of tile 0 and of tile 1
 //   warp 18         copies Q, K and V by tensor maps into a ring of stages
+//   warp 19         walks the run and hands out its blocks
 //
 // Tensor memory: two S buffers of 64 columns for each tile (P over the first 32
 // of its own), O0, O1 (head_dim columns each).  S of step j + 2 is issued behind
@@ -47,8 +57,13 @@ namespace pre {
 
 constexpr int kM = 128;        // q rows of a tile
 constexpr int kN = kPage;      // key rows of a step
-constexpr int kThreads = 640;  // warp 19 only completes the last warpgroup
-constexpr int kMmaWarp = 16, kLoadWarp = 18;
+constexpr int kThreads = 640;
+constexpr int kMmaWarp = 16, kLoadWarp = 18, kPlanWarp = 19;
+constexpr int kGrid = 148;         // one CTA an SM
+constexpr int kBlockRows = 2 * kM;
+constexpr int kBlockCost = 192;    // what a block costs beside its rows, in rows
+constexpr int kRunCost = 8 * kN + kBlockCost;  // no more CTAs than have this much, or a block each
+constexpr int kJobs = 4;           // blocks handed out ahead
 constexpr uint32_t kTmemCols = 512;
 // The launch has 96 registers a thread; the four softmax warpgroups take what the
 // fifth does without.  (Calls that are not inlined do not go with it: ptxas
@@ -68,9 +83,9 @@ struct Params {
   int window;
   const float* sinks;
   float scale_log2;
-  int n_splits;
-  float* part_o;   // [n_splits][n_tokens][n_q_heads][head_dim]
-  float* part_ml;  // [n_splits][n_tokens][n_q_heads][2]
+  float* part_o;   // [2 * kGrid][256 rows of a block][head_dim]
+  float* part_ml;  // [2 * kGrid][256][2]
+  int4* parts;     // [2 * kGrid]: first token, tokens, kv head, 1: written, 3: and the block's last
   uint16_t* out;
   uint32_t* status;
 };
@@ -79,19 +94,28 @@ template <int D>
 struct Layout {
   static constexpr int kQ = kM * D * 2;      // bytes of a Q tile
   static constexpr int kStage = kN * D * 2;  // K or V of a page
-  static constexpr int kStages = D == 128 ? 10 : 16;
+  static constexpr int kStages = D == 128 ? 9 : 16;
   static constexpr int kQCol = kM * 128;     // a 64-lane column block of a Q tile
   static constexpr int kCol = kN * 128;      // and of a page
   static constexpr int kRing = 2 * kQ;
-  static constexpr int kBars = kRing + kStages * kStage;
-  // full[kStages], empty[kStages], S full [2][2], P full [2][2], PV done [2], Q full, drain [2], reference [2][4], O complete [2]
-  static constexpr int kBarEmpty = 8 * kStages, kBarS = 16 * kStages, kBarP = kBarS + 32, kBarPv = kBarP + 32,
-                       kBarQ = kBarPv + 16, kBarDrain = kBarQ + 8;
-  static constexpr int kBarRef = kBarDrain + 16;
-  static constexpr int kBarO = kBarRef + 64;
-  static constexpr int kMisc = kBars + kBarO + 16;  // TMEM address, abort flag, found, scan
-  static constexpr int kRef = kMisc + 128;           // exponent references [2][128]
-  static constexpr int kTotal = kRef + 1024 + 1024;  // slack for the 1024-byte alignment
+  static constexpr int kEnds = kRing + kStages * kStage;  // [2][2 tiles][2 sets][128] reference and sum at a block's end
+  static constexpr int kRef = kEnds + 8192;               // exponent references [2][128]
+  static constexpr int kJob = kRef + 1024;                // [kJobs] of 64 bytes
+  static constexpr int kBars = kJob + 64 * kJobs;
+  static constexpr int kBarEmpty = 8 * kStages;   // full[kStages], empty[kStages]
+  static constexpr int kBarS = 16 * kStages;      // S full [2][2]
+  static constexpr int kBarP = kBarS + 32;        // P full [2][2]
+  static constexpr int kBarPv = kBarP + 32;       // O += P V of a step done [2]
+  static constexpr int kBarO = kBarPv + 16;       // O of a block done [2]
+  static constexpr int kBarOFree = kBarO + 16;    // and read [2]
+  static constexpr int kBarEnds = kBarOFree + 16; // both sets' ends written [2]
+  static constexpr int kBarRef = kBarEnds + 16;   // reference of a step written [2][4]
+  static constexpr int kBarQ = kBarRef + 64;      // Q full, Q free
+  static constexpr int kBarJob = kBarQ + 16;      // job full[kJobs], free[kJobs]
+  static constexpr int kBarDrain = kBarJob + 16 * kJobs;  // [2]
+  static constexpr int kMisc = kBars + kBarDrain + 16;    // TMEM address, abort flag, start of the run
+  static constexpr int kScan = kMisc + 32;                // [20] sums of the warps: costs, blocks
+  static constexpr int kTotal = kScan + 12 * 20 + 1024;   // slack for the 1024-byte alignment
 };
 
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -188,27 +212,69 @@ __device__ __forceinline__ float weights(const uint32_t (&x)[kN], uint32_t ts, u
   return __uint_as_float((uint32_t)sum) + __uint_as_float((uint32_t)(sum >> 32));
 }
 
-// Place of step j's K and V in the ring's order K0 K1 V0 K2 V1 K3 ...
-__device__ __forceinline__ int k_place(int j) { return j == 0 ? 0 : 2 * j - 1; }
-__device__ __forceinline__ int v_place(int j) { return 2 * j + 2; }
-
 // The new tokens of sequence s in q: [begin, end), cut to what q holds.
 __device__ __forceinline__ int2 new_tokens(const Params& p, int s) {
   const int a = min(max(__ldg(p.cu_q + s), 0), p.n_tokens);
   return make_int2(a, min(max(__ldg(p.cu_q + s + 1), a), p.n_tokens));
 }
 
-// What a CTA works on, the same for all of its threads.
-struct Work {
-  int head;         // kv head
-  int seq;
-  int token;        // first token (row of q)
-  int tokens;       // tokens of both tiles
-  int pos;          // position of the first token, may be negative
-  int len;          // rows of the sequence
-  int step0, steps; // pages of this CTA's split
-  int steps0;       // of which tile 0 needs the first ones only
+// A sequence's blocks for one kv head.  Block i has the tokens [i span, (i + 1)
+// span) and sees the rows [begin(i), end(i)); it weighs as many and kBlockCost.
+struct Blocks {
+  int token, tokens, len, pos, span, window, count;
+  __device__ __forceinline__ void init(const Params& p, int s) {
+    const int2 t = new_tokens(p, s);
+    token = t.x;
+    tokens = t.y - t.x;
+    len = min(max(__ldg(p.kv_lens + s), 0), (int)p.pt_stride * kPage);
+    pos = len - tokens;  // position of the first token, may be negative
+    span = 2 * p.tile_tokens;
+    window = p.window;
+    count = (tokens + span - 1) / span;
+  }
+  __device__ __forceinline__ int end(int i) const { return max(0, pos + min(tokens, (i + 1) * span)); }
+  __device__ __forceinline__ int begin(int i) const { return window > 0 ? max(0, pos + i * span - window + 1) : 0; }
+  __device__ __forceinline__ long long cost(int i) const { return kBlockCost + end(i) - min(begin(i), end(i)); }
+  // sum over i < n of max(0, a + i span)
+  __device__ __forceinline__ long long ramp(long long n, long long a) const {
+    const long long i0 = a > 0 ? 0 : (-a) / span + 1;  // the first above zero
+    if (i0 >= n) return 0;
+    return (n - i0) * a + span * (n * (n - 1) / 2 - i0 * (i0 - 1) / 2);
+  }
+  // cost of the blocks before n
+  __device__ __forceinline__ long long before(int n) const {
+    long long c = (long long)n * kBlockCost + ramp(n, (long long)pos + span);
+    if (window > 0) c -= ramp(n, (long long)pos - window + 1);
+    if (n == count && n > 0) c -= (long long)pos + (long long)n * span - len;  // the last one may be short
+    return c;
+  }
+  __device__ __forceinline__ int first_step(int i) const { return begin(i) / kN; }
+  __device__ __forceinline__ int steps(int i) const {
+    return end(i) > begin(i) ? (end(i) + kN - 1) / kN - begin(i) / kN : 0;
+  }
 };
+// Where a cut at `at` of a block's cost goes: its step.  Blocks of up to 8 steps
+// stay whole, longer ones are not cut within 4 of their ends.
+__device__ __forceinline__ int cut_step(long long at, long long cost, int steps) {
+  if (at <= 0) return 0;
+  if (at >= cost) return steps;
+  if (steps <= 8) return 2 * at >= cost ? steps : 0;
+  const int k = (int)(at * steps / cost);
+  return k < 4 ? 0 : steps - k < 4 ? steps : k;
+}
+
+// A block, or a part of its steps, as handed to the warps.
+struct Job {
+  int head, seq;
+  int token;          // first token (row of q)
+  int tokens;         // of both tiles
+  int pos;            // position of the first token, may be negative
+  int len;            // rows of the sequence
+  int step0, steps;   // pages; steps < 0: no more jobs
+  int steps0;         // of which tile 0 needs the first ones only
+  int slot;           // of the partial result, -1: the whole block
+};
+static_assert(sizeof(Job) <= 64, "job slot");
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -220,8 +286,10 @@ prefill_kernel(const Params p, const __grid_constant__ CUtensorMap map, const __
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kMisc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kMisc + 4);
-  int* found = reinterpret_cast<int*>(smem + L::kMisc + 8);  // sequence, block within it
-  int* scan = reinterpret_cast<int*>(smem + L::kMisc + 16);  // [20] per warp
+  volatile int* start_seq = reinterpret_cast<volatile int*>(smem + L::kMisc + 8);
+  volatile long long* start_off = reinterpret_cast<volatile long long*>(smem + L::kMisc + 16);
+  long long* scan = reinterpret_cast<long long*>(smem + L::kScan);
+  int* block_sums = reinterpret_cast<int*>(smem + L::kScan + 160);
 
   if (tid == 0) {
     for (int i = 0; i < L::kStages; ++i) {
@@ -232,16 +300,21 @@ prefill_kernel(const Params p, const __grid_constant__ CUtensorMap map, const __
       mbar_init(bars + L::kBarS + 8 * i, 1);
       mbar_init(bars + L::kBarP + 8 * i, 128);
     }
-    mbar_init(bars + L::kBarPv, 1);
-    mbar_init(bars + L::kBarPv + 8, 1);
-    mbar_init(bars + L::kBarQ, 1);
-    mbar_init(bars + L::kBarDrain, 1);
-    mbar_init(bars + L::kBarDrain + 8, 1);
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(bars + L::kBarPv + 8 * t, 1);
+      mbar_init(bars + L::kBarO + 8 * t, 1);
+      mbar_init(bars + L::kBarOFree + 8 * t, 8);  // warps of a tile
+      mbar_init(bars + L::kBarEnds + 8 * t, 8);
+      mbar_init(bars + L::kBarDrain + 8 * t, 1);
+    }
     for (int i = 0; i < 8; ++i) mbar_init(bars + L::kBarRef + 8 * i, 1);
-    mbar_init(bars + L::kBarO, 1);
-    mbar_init(bars + L::kBarO + 8, 1);
+    mbar_init(bars + L::kBarQ, 1);
+    mbar_init(bars + L::kBarQ + 8, 2);
+    for (int i = 0; i < kJobs; ++i) {
+      mbar_init(bars + L::kBarJob + 8 * i, 1);
+      mbar_init(bars + L::kBarJob + 8 * (kJobs + i), kPlanWarp);  // every other warp
+    }
     *abort_flag = 0;
-    found[0] = -1;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&map) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&qmap) : "memory");
@@ -263,36 +336,56 @@ prefill_kernel(const Params p, const __grid_constant__ CUtensorMap map, const __
   grid_dependency_wait();
   grid_launch_dependents();
 
-  // ---- which sequence and tokens: blocks of two tiles, the last tokens first
-  const int span = 2 * p.tile_tokens;
-  const int rank = blockIdx.x / p.cache.n_kv_heads;
+  // ---- this CTA's run: [u0, u1) of the cost of all blocks
+  long long u0, u1;
   {
     const int per = (p.n_seq + kThreads - 1) / kThreads;
     const int s_begin = min(tid * per, p.n_seq), s_end = min(s_begin + per, p.n_seq);
-    int mine = 0;
+    long long mine = 0, blocks = 0;
     for (int s = s_begin; s < s_end; ++s) {
-      const int2 t = new_tokens(p, s);
-      mine += (t.y - t.x + span - 1) / span;
+      Blocks b;
+      b.init(p, s);
+      mine += b.before(b.count) * p.cache.n_kv_heads;
+      blocks += (long long)b.count * p.cache.n_kv_heads;
+      if (blockIdx.x == 0 && (b.len != __ldg(p.kv_lens + s) || b.token != __ldg(p.cu_q + s) ||
+                              b.token + b.tokens != __ldg(p.cu_q + s + 1) || (s == 0 && b.token != 0) ||
+                              (s == p.n_seq - 1 && b.token + b.tokens != p.n_tokens)))
+        set_status(p.status, RKV_ERR_INDEX_OUT_OF_RANGE);
     }
-    int upto = mine;
+    // the blocks count up to one for each CTA only, beside the cost in one number
+    blocks = min(blocks, (long long)kGrid);
+    long long upto = mine;
+    int many = (int)blocks;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, upto, o);
+      const long long v = __shfl_up_sync(0xffffffffu, upto, o);
       if (lane >= o) upto += v;
+      many += __shfl_xor_sync(0xffffffffu, many, o);
     }
     if (lane == 31) scan[warp] = upto;
+    if (lane == 0) block_sums[warp] = many;
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    for (int w = 0; w < warp; ++w) upto += scan[w];
-    int at = upto - mine;
-    if (rank >= at && rank < upto) {
+    long long total = 0;
+    many = 0;
+    for (int i = 0; i < kThreads / 32; ++i) {
+      if (i < warp) upto += scan[i];
+      total += scan[i];
+      many += block_sums[i];
+    }
+    const long long ctas = min((long long)gridDim.x, max((long long)many, total / kRunCost));
+    u0 = blockIdx.x < ctas ? blockIdx.x * total / ctas : total;
+    u1 = blockIdx.x < ctas ? (blockIdx.x + 1) * total / ctas : total;
+    long long at = upto - mine;
+    if (u0 < u1 && u0 >= at && u0 < upto) {
       for (int s = s_begin; s < s_end; ++s) {
-        const int2 t = new_tokens(p, s);
-        const int n = (t.y - t.x + span - 1) / span;
-        if (rank < at + n) {
-          found[0] = s;
-          found[1] = n - 1 - (rank - at);
+        Blocks b;
+        b.init(p, s);
+        const long long n = b.before(b.count) * p.cache.n_kv_heads;
+        if (u0 < at + n) {
+          *start_seq = s;
+          *start_off = u0 - at;
           break;
         }
         at += n;
@@ -301,42 +394,104 @@ prefill_kernel(const Params p, const __grid_constant__ CUtensorMap map, const __
     __syncthreads();
   }
   const uint32_t tmem = *tmem_slot;
-  Work w;
-  w.seq = found[0];
-  w.steps = w.steps0 = 0;
-  if (w.seq >= 0) {
-    const int2 t = new_tokens(p, w.seq);
-    w.head = blockIdx.x % p.cache.n_kv_heads;
-    const int first = found[1] * span;
-    w.token = t.x + first;
-    w.tokens = min(span, t.y - t.x - first);
-    const int given = __ldg(p.kv_lens + w.seq), most = (int)p.pt_stride * kPage;
-    w.len = min(max(given, 0), most);
-    w.pos = w.len - (t.y - t.x) + first;
-    const int end = w.pos + w.tokens;  // rows [.., end) are seen
-    const int begin = p.window > 0 ? max(0, w.pos - p.window + 1) : 0;
-    const int s0 = begin / kN, s1 = end > 0 ? (end + kN - 1) / kN : 0;
-    const int per = (max(0, s1 - s0) + p.n_splits - 1) / p.n_splits;
-    w.step0 = s0 + blockIdx.y * per;
-    w.steps = max(0, min(per, s1 - w.step0));
-    const int end0 = w.pos + min(w.tokens, p.tile_tokens);
-    w.steps0 = max(0, min(w.steps, (end0 > 0 ? (end0 + kN - 1) / kN : 0) - w.step0));
-    if (tid == 0 && (given != w.len || __ldg(p.cu_q) != 0 || __ldg(p.cu_q + p.n_seq) != p.n_tokens ||
-                     t.x != __ldg(p.cu_q + w.seq) || t.y != __ldg(p.cu_q + w.seq + 1)))
-      set_status(p.status, RKV_ERR_INDEX_OUT_OF_RANGE);
-  }
-  const int tiles = w.tokens > p.tile_tokens ? 2 : 1;
+  const Job* jobs = reinterpret_cast<const Job*>(smem + L::kJob);
+  // The next job, copied; false after the last one or when the CTA gives up.
+  int n_jobs = 0;
+  auto next_job = [&](Job& w, bool& ok) {
+    const int at = n_jobs % kJobs;
+    ok = __all_sync(0xffffffffu, mbar_wait(bars + L::kBarJob + 8 * at, (n_jobs / kJobs) & 1, abort_flag));
+    if (!ok) return false;
+    w = jobs[at];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bars + L::kBarJob + 8 * (kJobs + at));
+    ++n_jobs;
+    return w.steps >= 0;
+  };
+  // A warp that gives up says so; the others' waits end with it.
+  auto give_up = [&]() {
+    *abort_flag = 1;
+    set_status(p.status, RKV_ERR_CUDA);
+  };
 
   if (warp >= kMmaWarp) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
-    if (warp < kMmaWarp + 2 && w.steps > 0) {
+    if (warp == kPlanWarp) {
+      // ---------------------------------------------------------------- planner
+      if (lane == 0) {
+        Job* out = reinterpret_cast<Job*>(smem + L::kJob);
+        bool ok = true;
+        int n = 0;
+        auto hand_out = [&](const Job& w) {
+          const int at = n % kJobs;
+          // as long as the work before takes: twenty of the usual limits
+          for (int i = 0; n >= kJobs && !(ok = mbar_wait(bars + L::kBarJob + 8 * (kJobs + at), (n / kJobs - 1) & 1, abort_flag)); ++i)
+            if (i == 20 || *abort_flag) return;
+          out[at] = w;
+          mbar_arrive(bars + L::kBarJob + 8 * at);
+          ++n;
+        };
+        int4 first = make_int4(0, 0, 0, 0), last = first;  // what the two slots hold
+        long long left = u1 - u0;
+        if (left > 0) {
+          int s = *start_seq;
+          long long off = *start_off;
+          for (; left > 0 && ok; ++s, off = 0) {
+            Blocks b;
+            b.init(p, s);
+            const long long per_head = b.before(b.count);
+            if (per_head == 0) continue;
+            int head = (int)(off / per_head);
+            off -= head * per_head;
+            int lo = 0, hi = b.count;  // the block that holds `off`
+            while (hi - lo > 1) {
+              const int mid = (lo + hi) / 2;
+              if (b.before(mid) <= off) lo = mid;
+              else hi = mid;
+            }
+            long long x = off - b.before(lo);
+            for (; head < p.cache.n_kv_heads && left > 0 && ok; ++head, lo = 0) {
+              for (int i = lo; i < b.count && left > 0 && ok; ++i, x = 0) {
+                const long long cost = b.cost(i), stop = min(cost, x + left);
+                const int steps = b.steps(i), k0 = cut_step(x, cost, steps), k1 = cut_step(stop, cost, steps);
+                if (k1 > k0 || (steps == 0 && x == 0)) {
+                  Job w;
+                  w.head = head;
+                  w.seq = s;
+                  w.token = b.token + i * b.span;
+                  w.tokens = min(b.span, b.tokens - i * b.span);
+                  w.pos = b.pos + i * b.span;
+                  w.len = b.len;
+                  w.step0 = b.first_step(i) + k0;
+                  w.steps = k1 - k0;
+                  const int end0 = w.pos + min(w.tokens, p.tile_tokens);
+                  w.steps0 = max(0, min(w.steps, (end0 > 0 ? (end0 + kN - 1) / kN : 0) - w.step0));
+                  w.slot = -1;
+                  if (k1 - k0 < steps) {
+                    w.slot = 2 * blockIdx.x + (k0 == 0);
+                    (k0 == 0 ? last : first) = make_int4(w.token, w.tokens, head, k1 == steps ? 3 : 1);
+                  }
+                  hand_out(w);
+                }
+                left -= stop - x;
+              }
+            }
+          }
+        }
+        p.parts[2 * blockIdx.x] = first;
+        p.parts[2 * blockIdx.x + 1] = last;
+        Job w = {};
+        w.steps = -1;
+        if (ok) hand_out(w);
+        if (!ok) give_up();
+      }
+      __syncwarp();
+    } else if (warp < kMmaWarp + 2) {
       // ----------------------------------------------------------- MMA issuers
       // The whole warp waits, so that it stays converged; one lane issues.
       constexpr uint32_t kType = T::kCode == RKV_GQA_BF16 ? (1u << 7) | (1u << 10) : 0u;
       constexpr uint32_t kIdescS = (1u << 4) | kType | ((kN >> 3) << 17) | ((kM >> 4) << 24);
       constexpr uint32_t kIdescO = (1u << 4) | kType | (1u << 16) | ((D >> 3) << 17) | ((kM >> 4) << 24);
       const int t = warp - kMmaWarp;
-      const int steps = t == tiles - 1 ? w.steps : t < tiles ? w.steps0 : 0;
       const uint64_t qd = sw128_desc(base + t * L::kQ, 16, 1024);
       const uint64_t kd0 = sw128_desc(base + L::kRing, 16, 1024), vd0 = sw128_desc(base + L::kRing, L::kCol, 1024);
       const uint32_t ts = tmem + t * 128, to = tmem + 256 + t * D;
@@ -354,107 +509,116 @@ prefill_kernel(const Params p, const __grid_constant__ CUtensorMap map, const __
       auto full = [&](const Place& at) {
         return (bool)__all_sync(0xffffffffu, mbar_wait(bars + 8 * at.st, at.ph, abort_flag));
       };
-      // S of step j (one lane)
-      auto qk = [&](const Place& at, int j) {
+      // S of the tile's step n (one lane)
+      auto qk = [&](const Place& at, int n) {
         const uint64_t kd = kd0 + (uint64_t)((at.st * L::kStage) >> 4);
-        const uint32_t d = ts + (j & 1) * 64;
+        const uint32_t d = ts + (n & 1) * 64;
 #pragma unroll
         for (int k = 0; k < D / 16; ++k)
           mma_ss(d, qd + (uint64_t)(((k >> 2) * L::kQCol + (k & 3) * 32) >> 4),
                  kd + (uint64_t)(((k >> 2) * L::kCol + (k & 3) * 32) >> 4), kIdescS, k > 0);
-        mma_commit(bars + L::kBarS + 16 * t + 8 * (j & 1));
+        mma_commit(bars + L::kBarS + 16 * t + 8 * (n & 1));
         mma_commit(bars + L::kBarEmpty + 8 * at.st);
       };
-      bool ok = __all_sync(0xffffffffu, mbar_wait(bars + L::kBarQ, 0, abort_flag));
-      Place kp = {0, 0u}, vp = {2, 0u};
-      for (int j = 0; ok && j < 2 && j < w.steps; ++j, kp.skip(j)) {  // places 0, 1, 3
-        ok = full(kp);
-        if (!ok) break;
-        if (elect_one()) {
-          if (j < steps) qk(kp, j);
-          else mbar_arrive(bars + L::kBarEmpty + 8 * kp.st);
-        }
+      Place kp = {0, 0u};
+      int n = 0;       // steps of this tile so far: of step j of a job, n + j
+      int n_q = 0;     // jobs with steps
+      int n_o = 0;     // of which this tile had some
+      Job w;
+      bool ok = true;
+      while (next_job(w, ok)) {
+        if (w.steps == 0) continue;
+        const int tiles = w.tokens > p.tile_tokens ? 2 : 1;
+        const int steps = t == tiles - 1 ? w.steps : t < tiles ? w.steps0 : 0;
+        ok = __all_sync(0xffffffffu, mbar_wait(bars + L::kBarQ, n_q & 1, abort_flag));
+        // K and V lie in the ring in the order K0 K1 V0 K2 V1 ... V of the last step
+        Place vp = kp;
+        vp.skip(w.steps > 1 ? 2 : 1);
+        if (steps == 0 && elect_one()) mbar_arrive(bars + L::kBarQ + 8);
         __syncwarp();
-      }
-      for (int j = 0; ok && j < w.steps; ++j, vp.skip(2), kp.skip(2)) {
-        ok = full(vp) && (j + 2 >= w.steps || full(kp));
-        if (!ok) break;
-        const int past = w.len - (w.step0 + j) * kN;  // first row past the sequence's end: zeros there (both warps do it)
-        if (past < kN) {
-          for (int i = lane; i < (kN - past) * (D / 8); i += 32) {
-            const int r = past + i / (D / 8), c = i % (D / 8);
-            *reinterpret_cast<uint4*>(smem + L::kRing + vp.st * L::kStage + (c >> 3) * L::kCol + r * 128 +
-                                      (((c & 7) ^ (r & 7)) << 4)) = make_uint4(0, 0, 0, 0);
-          }
-          fence_proxy_async();
-          __syncwarp();
-        }
-        if (j >= steps) {  // the other tile's steps
+        for (int j = 0; ok && j < 2 && j < w.steps; ++j) {  // places 0 and 1
+          ok = full(kp);
+          if (!ok) break;
           if (elect_one()) {
-            mbar_arrive(bars + L::kBarEmpty + 8 * vp.st);
-            if (j + 2 < w.steps) mbar_arrive(bars + L::kBarEmpty + 8 * kp.st);
+            if (j < steps) qk(kp, n + j);
+            else mbar_arrive(bars + L::kBarEmpty + 8 * kp.st);
+            if (j == steps - 1) mma_commit(bars + L::kBarQ + 8);
           }
           __syncwarp();
-          continue;
+          kp.skip(j + 1);  // to 1, then 3
         }
-        ok = __all_sync(0xffffffffu, mbar_wait(bars + L::kBarP + 16 * t + 8 * (j & 1), (j >> 1) & 1, abort_flag));
-        if (!ok) break;
-        tc_fence_after();
-        if (elect_one()) {
-          const uint64_t vd = vd0 + (uint64_t)((vp.st * L::kStage) >> 4);
-          const uint32_t pa = ts + (j & 1) * 64;
+        if (w.steps == 1) kp.skip(1);  // past V0
+        for (int j = 0; ok && j < w.steps; ++j) {
+          ok = full(vp) && (j + 2 >= w.steps || full(kp));
+          if (!ok) break;
+          const int past = w.len - (w.step0 + j) * kN;  // first row past the sequence's end: zeros there (both warps do it)
+          if (past < kN) {
+            for (int i = lane; i < (kN - past) * (D / 8); i += 32) {
+              const int r = past + i / (D / 8), c = i % (D / 8);
+              *reinterpret_cast<uint4*>(smem + L::kRing + vp.st * L::kStage + (c >> 3) * L::kCol + r * 128 +
+                                        (((c & 7) ^ (r & 7)) << 4)) = make_uint4(0, 0, 0, 0);
+            }
+            fence_proxy_async();
+            __syncwarp();
+          }
+          if (j < steps) {
+            // the softmax warps have read the O before this one
+            if (j == 0 && n_o > 0)
+              ok = __all_sync(0xffffffffu, mbar_wait(bars + L::kBarOFree + 8 * t, (n_o - 1) & 1, abort_flag));
+            ok = ok && __all_sync(0xffffffffu, mbar_wait(bars + L::kBarP + 16 * t + 8 * ((n + j) & 1),
+                                                         ((n + j) >> 1) & 1, abort_flag));
+            if (!ok) break;
+            tc_fence_after();
+          }
+          if (elect_one()) {
+            if (j < steps) {
+              const uint64_t vd = vd0 + (uint64_t)((vp.st * L::kStage) >> 4);
+              const uint32_t pa = ts + ((n + j) & 1) * 64;
 #pragma unroll
-          for (int k = 0; k < kN / 16; ++k)
-            mma_ts(to, pa + 8 * k, vd + (uint64_t)((k * 2048) >> 4), kIdescO, (j > 0 || k > 0) ? 1u : 0u);
-          mma_commit(bars + L::kBarPv + 8 * t);
-          if (j == steps - 1) mma_commit(bars + L::kBarO + 8 * t);
-          mma_commit(bars + L::kBarEmpty + 8 * vp.st);
-          if (j + 2 < steps) qk(kp, j + 2);
-          else if (j + 2 < w.steps) mbar_arrive(bars + L::kBarEmpty + 8 * kp.st);
+              for (int k = 0; k < kN / 16; ++k)
+                mma_ts(to, pa + 8 * k, vd + (uint64_t)((k * 2048) >> 4), kIdescO, (j > 0 || k > 0) ? 1u : 0u);
+              mma_commit(bars + L::kBarPv + 8 * t);
+              if (j == steps - 1) mma_commit(bars + L::kBarO + 8 * t);
+              mma_commit(bars + L::kBarEmpty + 8 * vp.st);
+            } else {  // the other tile's steps
+              mbar_arrive(bars + L::kBarEmpty + 8 * vp.st);
+            }
+            if (j + 2 < steps) {
+              qk(kp, n + j + 2);
+              if (j + 2 == steps - 1) mma_commit(bars + L::kBarQ + 8);  // Q may be overwritten
+            } else if (j + 2 < w.steps) {
+              mbar_arrive(bars + L::kBarEmpty + 8 * kp.st);
+            }
+          }
+          __syncwarp();
+          vp.skip(j + 2 < w.steps ? 2 : 1);
+          if (j + 2 < w.steps) kp.skip(j + 3 < w.steps ? 2 : 1);
         }
-        __syncwarp();
+        if (!ok) break;
+        kp = vp;  // past the last V
+        n += steps;
+        n_q += 1;
+        n_o += steps > 0;
       }
-      if (!ok) {
-        *abort_flag = 1;
-        set_status(p.status, RKV_ERR_CUDA);
-      }
+      if (!ok) give_up();
       // every MMA is done before the tensor memory is freed
       if (elect_one()) mma_commit(bars + L::kBarDrain + 8 * t);
       __syncwarp();
       mbar_wait_copy(bars + L::kBarDrain + 8 * t, 0);
-    } else if (warp == kLoadWarp && w.steps > 0) {
+    } else if (warp == kLoadWarp) {
       // ---------------------------------------------------------------- loader
       const int rows_total = (int)row_base(p.cache, p.cache.n_layers, 0, 0, 0);  // out of range: zero rows
       const int v_off = p.cache.n_kv_heads * kPage;
-      if (lane == 0) {
-        mbar_expect_tx(bars + L::kBarQ, tiles * (D / 64) * used * 128);
-        for (int t = 0; t < tiles; ++t)
-          for (int c = 0; c < D / 64; ++c)
-            asm volatile(
-                "cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, "
-                "%4}], [%5];" ::"r"(base + t * L::kQ + c * L::kQCol),
-                "l"(&qmap), "r"(64 * c), "r"(w.head * p.group), "r"(w.token + t * p.tile_tokens), "r"(bars + L::kBarQ)
-                : "memory");
-      }
-      const int32_t* ids = p.page_table + w.seq * p.pt_stride + w.step0;
-      // cache rows of the pages of 32 steps, one a lane
-      auto rows_of = [&](int at) {
-        int row = rows_total;
-        if (at + lane < w.steps) {
-          const int id = __ldg(ids + at + lane);
-          if (id >= 0 && id < p.cache.n_pages) row = (int)row_base(p.cache, p.layer, id, 0, w.head);
-          else set_status(p.status, RKV_ERR_INDEX_OUT_OF_RANGE);
-        }
-        return row;
-      };
+      Job w;
       bool ok = true;
-      int filled = 0;  // places of the ring's order that were filled or skipped
-      auto fill = [&](int n, int y) {
+      int n_q = 0;   // Q loads
+      int n = 0;     // places of the ring filled
+      auto fill = [&](int y) {
         const int st = n % L::kStages;
         if (n >= L::kStages)
           ok = __all_sync(0xffffffffu, mbar_wait(bars + L::kBarEmpty + 8 * st, (n / L::kStages - 1) & 1, abort_flag));
         if (!ok) return;
-        filled = n + 1;
+        ++n;
         if (lane == 0) {
           const uint32_t full = bars + 8 * st, dst = base + L::kRing + st * L::kStage;
           mbar_expect_tx(full, L::kStage);
@@ -462,181 +626,236 @@ prefill_kernel(const Params p, const __grid_constant__ CUtensorMap map, const __
           for (int c = 0; c < D / 64; ++c) tma_load_2d(dst + c * L::kCol, &map, 64 * c, y, full);
         }
       };
-      int v_rows = rows_of(0), k_rows = v_rows;  // of the 32 steps that V and K are at
-      fill(0, __shfl_sync(0xffffffffu, k_rows, 0));
-      if (w.steps > 1) fill(1, __shfl_sync(0xffffffffu, k_rows, 1));
-      for (int j = 0; ok && j < w.steps; ++j) {
-        if (j > 0 && j % 32 == 0) v_rows = k_rows;
-        const int y = __shfl_sync(0xffffffffu, v_rows, j % 32);
-        fill(v_place(j), y == rows_total ? y : y + v_off);
-        if (!ok || j + 2 >= w.steps) continue;
-        if ((j + 2) % 32 == 0) k_rows = rows_of(j + 2);
-        fill(k_place(j + 2), __shfl_sync(0xffffffffu, k_rows, (j + 2) % 32));
+      while (next_job(w, ok)) {
+        if (w.steps == 0) continue;
+        const int32_t* ids = p.page_table + w.seq * p.pt_stride + w.step0;
+        // cache rows of the pages of 32 steps, one a lane
+        auto rows_of = [&](int at) {
+          int row = rows_total;
+          if (at + lane < w.steps) {
+            const int id = __ldg(ids + at + lane);
+            if (id >= 0 && id < p.cache.n_pages) row = (int)row_base(p.cache, p.layer, id, 0, w.head);
+            else set_status(p.status, RKV_ERR_INDEX_OUT_OF_RANGE);
+          }
+          return row;
+        };
+        int v_rows = rows_of(0), k_rows = v_rows;  // of the 32 steps that V and K are at
+        // Q, once the MMAs of the job before have read theirs (twenty of the usual limits: it may be a long one)
+        for (int i = 0; n_q > 0 && !(ok = __all_sync(0xffffffffu, mbar_wait(bars + L::kBarQ + 8, (n_q - 1) & 1, abort_flag))); ++i)
+          if (i == 20 || __any_sync(0xffffffffu, *abort_flag)) break;
+        if (!ok) break;
+        ++n_q;
+        if (lane == 0) {
+          const int tiles = w.tokens > p.tile_tokens ? 2 : 1;
+          mbar_expect_tx(bars + L::kBarQ, tiles * (D / 64) * used * 128);
+          for (int t = 0; t < tiles; ++t)
+            for (int c = 0; c < D / 64; ++c)
+              asm volatile(
+                  "cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, "
+                  "%4}], [%5];" ::"r"(base + t * L::kQ + c * L::kQCol),
+                  "l"(&qmap), "r"(64 * c), "r"(w.head * p.group), "r"(w.token + t * p.tile_tokens), "r"(bars + L::kBarQ)
+                  : "memory");
+        }
+        fill(__shfl_sync(0xffffffffu, k_rows, 0));
+        for (int j = 0; ok && j < w.steps; ++j) {  // K of step j + 1, V of step j
+          if (j + 1 < w.steps) {
+            if ((j + 1) % 32 == 0) k_rows = rows_of(j + 1);
+            fill(__shfl_sync(0xffffffffu, k_rows, (j + 1) % 32));
+            if (!ok) break;
+          }
+          const int y = __shfl_sync(0xffffffffu, v_rows, j % 32);
+          fill(y == rows_total ? y : y + v_off);
+          if ((j + 1) % 32 == 0) v_rows = k_rows;
+        }
+        if (!ok) break;
       }
-      if (!ok) {
-        *abort_flag = 1;
-        set_status(p.status, RKV_ERR_CUDA);
-      }
+      if (!ok) give_up();
       // every copy has landed before the CTA ends
-      mbar_wait_copy(bars + L::kBarQ, 0);
-      const int skipped = 2 * w.steps - 1;  // the place of the K after the last; with one step, of K1
-      for (int i = max(0, filled - L::kStages); i < filled; ++i)
-        if (i != skipped) mbar_wait_copy(bars + 8 * (i % L::kStages), (i / L::kStages) & 1);
+      if (n_q > 0) mbar_wait_copy(bars + L::kBarQ, (n_q - 1) & 1);
+      for (int i = max(0, n - L::kStages); i < n; ++i)
+        mbar_wait_copy(bars + 8 * (i % L::kStages), (i / L::kStages) & 1);
     }
   } else {
     // --------------------------------------------------------------- softmax
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
-    const int t = warp >> 3, b = (warp >> 2) & 1;      // tile, and which of its steps (and S buffers)
-    const int r = 32 * (warp & 3) + lane;              // row of the tile
-    const int token = t * p.tile_tokens + r / p.group; // of the CTA's tokens
-    const bool live = w.seq >= 0 && r < used && token < w.tokens;
+    const int t = warp >> 3, b = (warp >> 2) & 1;       // tile, and which of its S buffers (and so steps)
+    const int r = 32 * (warp & 3) + lane;               // row of the tile
+    const int row_token = t * p.tile_tokens + r / p.group;  // of a job's tokens
     const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
     const uint32_t ts = tmem + lanes + t * 128 + 64 * b;
     const uint32_t to = tmem + lanes + 256 + t * D;
-    const int steps = t < tiles - 1 ? w.steps0 : t < tiles ? w.steps : 0;  // a row past them sees nothing there
-    const int pos = w.pos + token;                  // this row's position
-    const int pos_min = w.pos + t * p.tile_tokens;  // the tile's first and last
-    const int pos_max = pos_min + p.tile_tokens - 1;
     const uint32_t ref_bar = bars + L::kBarRef + 32 * t + 8 * (warp & 3);
     volatile float* ref = reinterpret_cast<volatile float*>(smem + L::kRef) + 128 * t + r;
-    float m = -INFINITY;  // exponent reference of l
-    float l = 0.f;        // sum of the weights of this set's steps
-    bool ok = true;
     const unsigned long long c2 = dup2(p.scale_log2);
-    for (int j = b; j < steps; j += 2) {
-      if (!__all_sync(0xffffffffu, mbar_wait(bars + L::kBarS + 16 * t + 8 * b, (j >> 1) & 1, abort_flag))) {
-        ok = false;
-        break;
+    int n = 0;    // steps of this tile so far: of step j of a job, n + j
+    int n_o = 0;  // jobs in which the tile had some
+    bool ok = true;
+    for (int n_jobs = 0;; ++n_jobs) {
+      const int slot = n_jobs % kJobs;
+      const Job* job = jobs + slot;
+      const uint32_t job_free = bars + L::kBarJob + 8 * (kJobs + slot);
+      ok = __all_sync(0xffffffffu, mbar_wait(bars + L::kBarJob + 8 * slot, (n_jobs / kJobs) & 1, abort_flag));
+      if (!ok || job->steps < 0) break;
+      const int tiles = job->tokens > p.tile_tokens ? 2 : 1;
+      if (t >= tiles) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(job_free);
+        continue;
       }
-      tc_fence_after();
-      uint32_t x[kN];
-#pragma unroll
-      for (int i = 0; i < kN; i += 32) tmem_ld32(ts + i, x + i);
-      tmem_wait_ld();
-      const int key0 = (w.step0 + j) * kN;
-      const bool masked = key0 + kN - 1 > pos_min || (p.window > 0 && key0 <= pos_max - p.window);
-      if (masked) {
-        const int last = pos - key0, first = p.window > 0 ? last - p.window : -1;
-#pragma unroll
-        for (int i = 0; i < kN; ++i)
-          if (i > last || i <= first) x[i] = 0xff800000u;  // -inf
-      }
-      float t0 = __uint_as_float(x[0]), t1 = __uint_as_float(x[1]), t2 = __uint_as_float(x[2]),
-            t3 = __uint_as_float(x[3]);
-#pragma unroll
-      for (int i = 4; i < kN - 4; i += 8) {
-        t0 = fmax3(t0, __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
-        t1 = fmax3(t1, __uint_as_float(x[i + 2]), __uint_as_float(x[i + 3]));
-        t2 = fmax3(t2, __uint_as_float(x[i + 4]), __uint_as_float(x[i + 5]));
-        t3 = fmax3(t3, __uint_as_float(x[i + 6]), __uint_as_float(x[i + 7]));
-      }
-      t0 = fmax3(t0, __uint_as_float(x[kN - 4]), __uint_as_float(x[kN - 3]));
-      t1 = fmax3(t1, __uint_as_float(x[kN - 2]), __uint_as_float(x[kN - 1]));
-      const float top = fmaxf(fmax3(t0, t1, t2), t3) * p.scale_log2 - SoftmaxBias<T>::kBias;
-      // the reference that the step before left, and this step's
-      float was = m;
-      if (j > 0) {
-        if (!__all_sync(0xffffffffu, mbar_wait(ref_bar, (j - 1) & 1, abort_flag))) {
+      const int steps = t < tiles - 1 ? job->steps0 : job->steps;  // a row past them sees nothing there
+      const int row0 = job->step0 * kN - job->pos;                 // first row of step 0 from the first token's position
+      const int pos_min = t * p.tile_tokens;                       // the tile's first and last position from there
+      const int pos_max = pos_min + p.tile_tokens - 1;
+      float m = -INFINITY;  // exponent reference of l
+      float l = 0.f;        // sum of the weights of this set's steps
+      for (int j = (n ^ b) & 1; j < steps; j += 2) {
+        if (!__all_sync(0xffffffffu, mbar_wait(bars + L::kBarS + 16 * t + 8 * b, ((n + j) >> 1) & 1, abort_flag))) {
           ok = false;
           break;
         }
-        was = *ref;
-      }
-      const bool up = top > was + kLazyLog2 || (was == -INFINITY && top > -INFINITY);
-      const float now = up ? top : was;
-      *ref = now;
-      __syncwarp();
-      if (lane == 0) mbar_arrive(ref_bar);
-      if (__any_sync(0xffffffffu, now != m)) {  // it moved in this step or in the one before
-        l *= now == m ? 1.f : ex2(m - now);     // 0 from -inf
-        m = now;
-        if (j > 0 && __any_sync(0xffffffffu, up)) {
-          const float a = up ? ex2(was - now) : 1.f;
-          // O holds the steps up to j - 1 once their MMAs are done: S of this step was issued behind step j - 2's, and
-          // step j's wait for this warp, so the barrier is in phase j - 1 or just past it
-          if (!__all_sync(0xffffffffu, mbar_wait(bars + L::kBarPv + 8 * t, (j - 1) & 1, abort_flag))) {
+        tc_fence_after();
+        uint32_t x[kN];
+#pragma unroll
+        for (int i = 0; i < kN; i += 32) tmem_ld32(ts + i, x + i);
+        tmem_wait_ld();
+        const int key0 = row0 + j * kN;
+        if (key0 + kN - 1 > pos_min || (p.window > 0 && key0 <= pos_max - p.window)) {
+          const int last = row_token - key0, first = p.window > 0 ? last - p.window : -1;
+#pragma unroll
+          for (int i = 0; i < kN; ++i)
+            if (i > last || i <= first) x[i] = 0xff800000u;  // -inf
+        }
+        float t0 = __uint_as_float(x[0]), t1 = __uint_as_float(x[1]), t2 = __uint_as_float(x[2]),
+              t3 = __uint_as_float(x[3]);
+#pragma unroll
+        for (int i = 4; i < kN - 4; i += 8) {
+          t0 = fmax3(t0, __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
+          t1 = fmax3(t1, __uint_as_float(x[i + 2]), __uint_as_float(x[i + 3]));
+          t2 = fmax3(t2, __uint_as_float(x[i + 4]), __uint_as_float(x[i + 5]));
+          t3 = fmax3(t3, __uint_as_float(x[i + 6]), __uint_as_float(x[i + 7]));
+        }
+        t0 = fmax3(t0, __uint_as_float(x[kN - 4]), __uint_as_float(x[kN - 3]));
+        t1 = fmax3(t1, __uint_as_float(x[kN - 2]), __uint_as_float(x[kN - 1]));
+        const float top = fmaxf(fmax3(t0, t1, t2), t3) * p.scale_log2 - SoftmaxBias<T>::kBias;
+        // the reference that the step before left, and this step's
+        float was = m;
+        if (j > 0) {
+          if (!__all_sync(0xffffffffu, mbar_wait(ref_bar, (n + j - 1) & 1, abort_flag))) {
             ok = false;
             break;
           }
-          tc_fence_after();
+          was = *ref;
+        }
+        const bool up = top > was + kLazyLog2 || (was == -INFINITY && top > -INFINITY);
+        const float now = up ? top : was;
+        *ref = now;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(ref_bar);
+        if (__any_sync(0xffffffffu, now != m)) {  // it moved in this step or in the one before
+          l *= now == m ? 1.f : ex2(m - now);     // 0 from -inf
+          m = now;
+          if (j > 0 && __any_sync(0xffffffffu, up)) {
+            const float a = up ? ex2(was - now) : 1.f;
+            // O holds the steps up to j - 1 once their MMAs are done: S of this step was issued behind step j - 2's,
+            // and step j's wait for this warp, so the barrier is in that phase or just past it
+            if (!__all_sync(0xffffffffu, mbar_wait(bars + L::kBarPv + 8 * t, (n + j - 1) & 1, abort_flag))) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
 #pragma unroll 1
-          for (int c = 0; c < D; c += 16) {
-            uint32_t o[16];
-            tmem_ld16(to + c, o);
-            tmem_wait_ld();
+            for (int c = 0; c < D; c += 16) {
+              uint32_t o[16];
+              tmem_ld16(to + c, o);
+              tmem_wait_ld();
 #pragma unroll
-            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * a);
-            tmem_st16(to + c, o);
+              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * a);
+              tmem_st16(to + c, o);
+            }
           }
         }
+        const unsigned long long n2 = dup2(m == -INFINITY ? 0.f : -m);  // nothing seen yet: weights 0
+        l += weights<T>(x, ts, c2, n2);
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(bars + L::kBarP + 16 * t + 8 * b);
       }
-      const unsigned long long n2 = dup2(m == -INFINITY ? 0.f : -m);  // nothing seen yet: weights 0
-      l += weights<T>(x, ts, c2, n2);
-      tmem_wait_st();
-      tc_fence_before();
-      mbar_arrive(bars + L::kBarP + 16 * t + 8 * b);
-    }
-    if (ok && steps > 0) ok = __all_sync(0xffffffffu, mbar_wait(bars + L::kBarO + 8 * t, 0, abort_flag));
-    if (!ok) {
-      *abort_flag = 1;
-      set_status(p.status, RKV_ERR_CUDA);
-    }
-    tc_fence_after();
-    // ---- epilogue: both sets' sums together, then one row a thread, half of its lanes a set
-    if (w.seq >= 0 && t < tiles) {
-      if (steps > 0) {  // through the tile's Q, which no MMA needs any more
-        float2* ends = reinterpret_cast<float2*>(smem + t * L::kQ) + r;
-        ends[kM * b] = make_float2(m, l);
-        if (t == 0) asm volatile("bar.sync 1, 256;" ::: "memory");
-        else asm volatile("bar.sync 2, 256;" ::: "memory");
-        const float2 other = ends[kM * (1 - b)];
+      if (!ok) break;
+      // ---- epilogue: both sets' sums together, then one row a thread, half of its lanes a set
+      if (steps > 0) {
+        float2* ends = reinterpret_cast<float2*>(smem + L::kEnds) + 512 * (n_o & 1) + 256 * t + r;
+        ends[128 * b] = make_float2(m, l);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bars + L::kBarEnds + 8 * t);
+        ok = __all_sync(0xffffffffu, mbar_wait(bars + L::kBarEnds + 8 * t, n_o & 1, abort_flag)) &&
+             __all_sync(0xffffffffu, mbar_wait(bars + L::kBarO + 8 * t, n_o & 1, abort_flag));
+        if (!ok) break;
+        const float2 other = ends[128 * (1 - b)];
         const float mm = fmaxf(m, other.x);
         if (mm != -INFINITY) l = l * ex2(m - mm) + other.y * ex2(other.x - mm);
         m = mm;
+        tc_fence_after();
+        n += steps;
+        n_o += 1;
       }
-      const int head = w.head * p.group + r % p.group;
-      const int64_t row = (int64_t)(w.token + token) * p.n_q_heads + head;
-      const bool have = ok && steps > 0;
-      float f = 1.f;
-      float* part = nullptr;
-      if (p.n_splits > 1) {
-        const int64_t at = (int64_t)blockIdx.y * p.n_tokens * p.n_q_heads + row;
-        part = p.part_o + at * D;
-        if (live && b == 0) *reinterpret_cast<float2*>(p.part_ml + 2 * at) = make_float2(have ? m : -INFINITY, l);
-      } else if (live) {
+      // the rest of the job, read (and what the row needs worked out) only here: it would not fit beside S
+      int row = r;
+      asm volatile("" : "+r"(row));
+      const Job w = *job;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(job_free);
+      const int token = t * p.tile_tokens + row / p.group;
+      const bool live = row < used && token < w.tokens;
+      const bool seen = m != -INFINITY;  // a row that saw nothing: zeros, whatever O holds
+      const int head = w.head * p.group + row % p.group;
+      float f = seen ? 1.f : 0.f;
+      const int64_t at = (int64_t)w.slot * kBlockRows + t * kM + row;
+      if (w.slot >= 0) {
+        if (live && b == 0) *reinterpret_cast<float2*>(p.part_ml + 2 * at) = make_float2(m, l);
+      } else if (live && seen) {
         const float sink = p.sinks ? p.sinks[head] * 1.4426950408889634f : -INFINITY;
         const float top = fmaxf(m, sink);
         const float e = ex2(m - top);
-        f = m == -INFINITY ? 0.f : e / (l * e + ex2(sink - top));
+        f = e / (l * e + ex2(sink - top));
       }
-      const bool seen = have && m != -INFINITY;  // a row that saw nothing: zeros, whatever O holds
+      uint16_t* dst = p.out + ((int64_t)(w.token + token) * p.n_q_heads + head) * D;
 #pragma unroll 1
       for (int c = b * (D / 2); c < (b + 1) * (D / 2); c += 32) {
         uint32_t o[32];
-        if (have) {
+        if (steps > 0) {
           tmem_ld32(to + c, o);
           tmem_wait_ld();
+          if (c + 32 == (b + 1) * (D / 2)) {  // O may be overwritten
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bars + L::kBarOFree + 8 * t);
+          }
+        } else {  // set on every path: else it would live on through the next job
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = 0u;
         }
 #pragma unroll
         for (int i = 0; i < 32; ++i) o[i] = seen ? __float_as_uint(__uint_as_float(o[i]) * f) : 0u;
         if (!live) continue;
-        if (part) {
+        if (w.slot >= 0) {
+          if (seen)
 #pragma unroll
-          for (int i = 0; i < 32; i += 4)
-            *reinterpret_cast<uint4*>(part + c + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+            for (int i = 0; i < 32; i += 8)
+              st_stream32(p.part_o + at * D + c + i, make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]),
+                          make_uint4(o[i + 4], o[i + 5], o[i + 6], o[i + 7]));
         } else {
 #pragma unroll
-          for (int i = 0; i < 32; i += 8) {
-            uint4 v;
-            v.x = T::pack(__uint_as_float(o[i]), __uint_as_float(o[i + 1]));
-            v.y = T::pack(__uint_as_float(o[i + 2]), __uint_as_float(o[i + 3]));
-            v.z = T::pack(__uint_as_float(o[i + 4]), __uint_as_float(o[i + 5]));
-            v.w = T::pack(__uint_as_float(o[i + 6]), __uint_as_float(o[i + 7]));
-            *reinterpret_cast<uint4*>(p.out + row * D + c + i) = v;
+          for (int i = 0; i < 32; i += 16) {
+            uint32_t v[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = T::pack(__uint_as_float(o[i + 2 * k]), __uint_as_float(o[i + 2 * k + 1]));
+            // 32 bytes a lane: the lanes' rows are apart, and the store unit takes one of them a clock
+            st_stream32(dst + c + i, make_uint4(v[0], v[1], v[2], v[3]), make_uint4(v[4], v[5], v[6], v[7]));
           }
         }
       }
     }
+    if (!ok) give_up();
   }
   tc_fence_before();
   __syncthreads();
@@ -645,34 +864,46 @@ prefill_kernel(const Params p, const __grid_constant__ CUtensorMap map, const __
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
 }
 
-// Joins the splits of one (token, q head) a warp, in their order.
+// Joins the parts of the block whose first part is the end of run c, in the
+// order of their rows: slot 2 c + 1, then slot 2 c' of the runs after it up to the
+// block's last part.  A warp a row, 32 rows a CTA.
 template <typename T, int D>
-__global__ void __launch_bounds__(128) join_kernel(const Params p) {
+__global__ void __launch_bounds__(256) join_kernel(const Params p) {
   grid_dependency_wait();
-  const int64_t rows = (int64_t)p.n_tokens * p.n_q_heads;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (row >= rows) return;
-  const int lane = threadIdx.x & 31;
-  const int head = (int)(row % p.n_q_heads);
-  const float sink = p.sinks ? p.sinks[head] * 1.4426950408889634f : -INFINITY;
-  float top = sink;
-  for (int i = 0; i < p.n_splits; ++i) top = fmaxf(top, p.part_ml[2 * (i * rows + row)]);
-  if (top == -INFINITY) top = 0.f;
-  float o[D / 32] = {};
-  float l = ex2(sink - top);
-  for (int i = 0; i < p.n_splits; ++i) {
-    const int64_t at = i * rows + row;
-    const float2 e = *reinterpret_cast<const float2*>(p.part_ml + 2 * at);
-    if (e.x == -INFINITY) continue;
-    const float w = ex2(e.x - top);
-    l += w * e.y;
+  const int c = blockIdx.x;
+  const int4 block = p.parts[2 * c + 1];
+  if (block.w == 0) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int i = warp; i < 32; i += 8) {
+    const int row = blockIdx.y * 32 + i, t = row / kM, r = row % kM;
+    const int token = t * p.tile_tokens + r / p.group;
+    if (r >= p.tile_tokens * p.group || token >= block.y) continue;
+    const int head = block.z * p.group + r % p.group;
+    const float sink = p.sinks ? p.sinks[head] * 1.4426950408889634f : -INFINITY;
+    float m = sink, l = sink == -INFINITY ? 0.f : 1.f;
+    float o[D / 32] = {};
+    for (int from = c; from < kGrid; ++from) {
+      const int slot = from == c ? 2 * c + 1 : 2 * from;
+      const int4 part = p.parts[slot];
+      // a run whose share of the block was cut away has none
+      if (part.w == 0 || part.x != block.x || part.z != block.z) continue;
+      const int64_t at = (int64_t)slot * kBlockRows + row;
+      const float2 e = *reinterpret_cast<const float2*>(p.part_ml + 2 * at);
+      if (e.x != -INFINITY) {
+        const float top = fmaxf(m, e.x);
+        const float a = ex2(m - top), w = ex2(e.x - top);  // 0 from -inf
+        l = l * a + e.y * w;
 #pragma unroll
-    for (int j = 0; j < D / 32; ++j) o[j] += w * p.part_o[at * D + D / 32 * lane + j];
+        for (int j = 0; j < D / 32; ++j) o[j] = o[j] * a + w * p.part_o[at * D + D / 32 * lane + j];
+        m = top;
+      }
+      if (part.w == 3) break;
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    uint32_t* dst = reinterpret_cast<uint32_t*>(p.out + ((int64_t)(block.x + token) * p.n_q_heads + head) * D) + D / 64 * lane;
+#pragma unroll
+    for (int j = 0; j < D / 64; ++j) dst[j] = T::pack(o[2 * j] * inv, o[2 * j + 1] * inv);
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-  for (int j = 0; j < D / 32; j += 2)
-    *reinterpret_cast<uint32_t*>(p.out + row * D + D / 32 * lane + j) = T::pack(o[j] * inv, o[j + 1] * inv);
 }
 
 template <typename T, int D>
@@ -691,19 +922,16 @@ static rkv_status launch(const Params& p, const CUtensorMap& map, const CUtensor
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
-  // every sequence rounds its tokens up to whole blocks: at most one more each
-  const int64_t blocks = ((int64_t)p.n_tokens / (2 * p.tile_tokens) + p.n_seq) * p.cache.n_kv_heads;
-  if (blocks > INT32_MAX) return fail(RKV_ERR_SHAPE_MISMATCH, "%s: too many tokens", what);
-  cfg.gridDim = dim3((unsigned)blocks, (unsigned)p.n_splits);
+  cfg.gridDim = dim3(kGrid);
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = Layout<D>::kTotal;
   cfg.stream = s;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
   cudaError_t e = cudaLaunchKernelEx(&cfg, prefill_kernel<T, D>, p, map, qmap);
-  if (e == cudaSuccess && p.n_splits > 1) {
-    cfg.gridDim = dim3((unsigned)(((int64_t)p.n_tokens * p.n_q_heads + 3) / 4));
-    cfg.blockDim = dim3(128);
+  if (e == cudaSuccess) {
+    cfg.gridDim = dim3(kGrid, kBlockRows / 32);
+    cfg.blockDim = dim3(256);
     cfg.dynamicSmemBytes = 0;
     e = cudaLaunchKernelEx(&cfg, join_kernel<T, D>, p);
   }
@@ -718,36 +946,17 @@ static rkv_status launch(const Params& p, const CUtensorMap& map, const CUtensor
 }  // namespace gqa
 }  // namespace rkv
 
-extern "C" int32_t rkv_gqa_prefill_splits(const rkv_gqa_view* cache, int64_t n_tokens, int32_t n_q_heads,
-                                          int32_t n_seq, int64_t pt_stride) {
-  if (!cache || n_tokens < 0 || n_q_heads < 1 || n_seq < 0 || pt_stride < 1 || cache->n_kv_heads < 1 ||
-      n_q_heads % cache->n_kv_heads != 0 || n_q_heads / cache->n_kv_heads > RKV_GQA_MAX_GROUP)
-    return -1;
-  // CTAs of the tokens alone; with fewer than half the SMs busy, cut the rows so that the SMs are covered, but
-  // not below 16 pages
-  const int64_t span = 2 * (128 / (n_q_heads / cache->n_kv_heads));
-  int64_t blocks = (n_tokens + span - 1) / span;
-  if (blocks < n_seq) blocks = n_seq;
-  blocks *= cache->n_kv_heads;
-  if (blocks == 0 || 2 * blocks > 148) return 1;
-  int64_t splits = 148 / blocks;
-  const int64_t most = pt_stride / 16;
-  if (splits > most) splits = most;
-  return splits < 1 ? 1 : splits > 64 ? 64 : (int32_t)splits;
-}
-
-extern "C" int64_t rkv_gqa_prefill_workspace_bytes(const rkv_gqa_view* cache, int64_t n_tokens, int32_t n_q_heads,
-                                                   int32_t n_splits) {
-  if (!cache || n_tokens < 0 || n_q_heads < 1 || n_splits < 1) return -1;
-  return n_splits == 1 ? 0 : n_splits * n_tokens * n_q_heads * (cache->head_dim + 2) * 4;
+extern "C" int64_t rkv_gqa_prefill_workspace_bytes(const rkv_gqa_view* cache) {
+  using namespace rkv::gqa::pre;
+  if (!cache || (cache->head_dim != 64 && cache->head_dim != 128)) return -1;
+  return (int64_t)2 * kGrid * (kBlockRows * (cache->head_dim + 2) * 4 + 16);
 }
 
 extern "C" rkv_status rkv_gqa_prefill(const rkv_gqa_view* cache, int32_t layer, const void* q, int64_t q_token_stride,
                                       int64_t q_head_stride, int64_t n_tokens, int32_t n_q_heads, const int32_t* cu_q,
                                       int32_t n_seq, const int32_t* page_table, int64_t pt_stride,
                                       const int32_t* kv_lens, int32_t window, const float* sinks, float softmax_scale,
-                                      int32_t n_splits, void* workspace, void* out, uint32_t* d_status,
-                                      rkv_stream_t stream) {
+                                      void* workspace, void* out, uint32_t* d_status, rkv_stream_t stream) {
   using namespace rkv;
   using namespace rkv::gqa;
   using namespace rkv::gqa::pre;
@@ -757,7 +966,6 @@ extern "C" rkv_status rkv_gqa_prefill(const rkv_gqa_view* cache, int32_t layer, 
   if ((st = check_heads(cache, n_q_heads, what)) != RKV_OK) return st;
   if (n_tokens < 0 || n_tokens > INT32_MAX / 2) return fail_shape("n_tokens", 0, n_tokens, "%s: bad n_tokens", what);
   if (n_seq < 0) return fail_shape("n_seq", 0, n_seq, "%s: n_seq < 0", what);
-  if (n_splits < 1 || n_splits > 64) return fail_shape("n_splits", 1, n_splits, "%s: 1 <= n_splits <= 64", what);
   if (n_tokens == 0 || n_seq == 0) {
     if (n_tokens > 0) return fail_shape("n_tokens", 0, n_tokens, "%s: tokens without a sequence", what);
     clear_error();
@@ -767,8 +975,8 @@ extern "C" rkv_status rkv_gqa_prefill(const rkv_gqa_view* cache, int32_t layer, 
                            pt_stride,  kv_lens, window, sinks,          softmax_scale, out,      d_status};
   if ((st = check_attend(args, what)) != RKV_OK) return st;
   if (!cu_q) return fail(RKV_ERR_INVALID_ARGUMENT, "%s: cu_q is required", what);
-  if (n_splits > 1 && (!workspace || !aligned(workspace, 16)))
-    return fail(RKV_ERR_INVALID_ARGUMENT, "%s: a 16-byte aligned workspace is required", what);
+  if (!workspace || !aligned(workspace, 32) || !aligned(out, 32))
+    return fail(RKV_ERR_INVALID_ARGUMENT, "%s: out and a workspace, both 32-byte aligned, are required", what);
   Params p;
   p.cache = *cache;
   p.layer = layer;
@@ -784,9 +992,9 @@ extern "C" rkv_status rkv_gqa_prefill(const rkv_gqa_view* cache, int32_t layer, 
   p.window = window;
   p.sinks = sinks;
   p.scale_log2 = (float)((double)softmax_scale * 1.4426950408889634);
-  p.n_splits = n_splits;
   p.part_o = static_cast<float*>(workspace);
-  p.part_ml = workspace ? p.part_o + n_splits * n_tokens * n_q_heads * cache->head_dim : nullptr;
+  p.part_ml = p.part_o + (int64_t)2 * kGrid * kBlockRows * cache->head_dim;
+  p.parts = reinterpret_cast<int4*>(p.part_ml + 2 * kGrid * kBlockRows * 2);
   p.out = static_cast<uint16_t*>(out);
   p.status = d_status;
   CUtensorMap map, qmap;

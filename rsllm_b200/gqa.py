@@ -106,6 +106,7 @@ class GqaKvPool:
                                  _DTYPES[cache.dtype])
         self._v = addressof(self.view)
         self._s = status.data_ptr()
+        self._prefill_ws = self.lib.rkv_gqa_prefill_workspace_bytes(self._v)
 
     # -- status ---------------------------------------------------------------
     def take_status(self, stream: torch.cuda.Stream | None = None) -> int:
@@ -210,7 +211,7 @@ class GqaKvPool:
     # -- attention -----------------------------------------------------------------
     def prefill(self, layer: int, q: torch.Tensor, cu_q: torch.Tensor, page_table: torch.Tensor, kv_lens: torch.Tensor,
                 softmax_scale: float | None = None, window: int = 0, sinks: torch.Tensor | None = None,
-                n_splits: int | None = None, out: torch.Tensor | None = None, workspace: torch.Tensor | None = None,
+                out: torch.Tensor | None = None, workspace: torch.Tensor | None = None,
                 stream: torch.cuda.Stream | None = None) -> torch.Tensor:
         """Causal attention of packed new tokens q ``[tokens, n_q_heads,
         head_dim]`` (sequence s: rows ``cu_q[s]`` to ``cu_q[s + 1]``) over the
@@ -223,14 +224,11 @@ class GqaKvPool:
         cu = self._need(cu_q, torch.int32, "cu_q", (n_seq + 1,))
         table, stride = self._table(page_table, n_seq)
         sink = 0 if sinks is None else self._need(sinks, torch.float32, "sinks", (heads,))
-        if n_splits is None:
-            n_splits = self.lib.rkv_gqa_prefill_splits(self._v, n, heads, n_seq, stride) if n and stride else 1
-        ws, wp = self._workspace(workspace, self.lib.rkv_gqa_prefill_workspace_bytes(self._v, n, heads, n_splits)
-                                 if n_splits > 1 else 0, stream)
+        ws, wp = self._workspace(workspace, self._prefill_ws, stream)
         out, op = self._out(out, q, "out", stream)
         scale = 1.0 / math.sqrt(self.head_dim) if softmax_scale is None else softmax_scale
         check(self.lib.rkv_gqa_prefill(self._v, layer, qp, q_ts, q_hs, n, heads, cu, n_seq, table, stride, lens, window,
-                                       sink, scale, n_splits, wp, op, self._s, self._stream(stream)), "prefill")
+                                       sink, scale, wp, op, self._s, self._stream(stream)), "prefill")
         return out
 
     def decode(self, layer: int, q: torch.Tensor, page_table: torch.Tensor, kv_lens: torch.Tensor,

@@ -51,15 +51,38 @@ def test_prefill(cuda, case):
     close(out, *b.want(window=window, sinks=sinks), dtype)
 
 
-@pytest.mark.parametrize("n_splits", [1, 2, 3, 7, 64])
-@pytest.mark.parametrize("window", [0, 200])
-def test_prefill_splits(cuda, n_splits, window):
-    """Any number of splits gives the same attention, splits without a row among them."""
-    b = Batch([10, 1, 33, 0, 130], [700, 1, 1500, 40, 100], 14, 2, 128, BF, seed=3)
+@pytest.mark.parametrize("window", [0, 200, 3000])
+@pytest.mark.parametrize("d,dtype", [(128, BF), (64, HF)])
+def test_prefill_parts(cuda, window, d, dtype):
+    """Few tokens and long prefixes: the rows of a token are shared out and joined, in more parts for some tokens than
+    for others; tokens without a row, short ones and one long prompt among them."""
+    q_lens, kv_lens = [10, 1, 33, 0, 130, 1, 700], [7000, 1, 15000, 40, 100, 0, 700]
+    b = Batch(q_lens, kv_lens, 14, 2, d, dtype, seed=3)
     pool = GqaKvPool.over(b.cache)
-    out = pool.prefill(0, b.q, b.cu_q, b.table, b.kv_lens, window=window, sinks=b.sinks, n_splits=n_splits)
+    ws = torch.full((1 << 26,), 255, dtype=torch.uint8, device=cuda)
+    out = pool.prefill(0, b.q, b.cu_q, b.table, b.kv_lens, window=window, sinks=b.sinks, workspace=ws)
     pool.check("prefill")
-    close(out, *b.want(window=window, sinks=True), BF)
+    close(out, *b.want(window=window, sinks=True), dtype)
+    again = pool.prefill(0, b.q, b.cu_q, b.table, b.kv_lens, window=window, sinks=b.sinks, workspace=ws)
+    assert torch.equal(out, again)
+
+
+@pytest.mark.parametrize("seed", range(12))
+def test_prefill_random_batches(cuda, seed):
+    """Drawn lengths, prefixes, heads, windows: every block boundary and cut somewhere."""
+    rng = np.random.default_rng(1000 + seed)
+    n = int(rng.integers(1, 40))
+    q_lens = [int(x) for x in rng.integers(0, [3, 60, 300, 900][seed % 4], n)]
+    q_lens[0] += 1
+    kv_lens = [q + int(x) for q, x in zip(q_lens, rng.integers(0, [1, 2000, 300, 64][seed // 3], n))]
+    hq, hkv = [(4, 4), (14, 2), (8, 1), (12, 4), (10, 2)][seed % 5]
+    dtype, d = (BF, HF)[seed % 2], (64, 128)[seed // 2 % 2]
+    window = [0, 0, 37, 500][seed % 4]
+    b = Batch(q_lens, kv_lens, hq, hkv, d, dtype, seed=seed)
+    pool = GqaKvPool.over(b.cache)
+    out = pool.prefill(0, b.q, b.cu_q, b.table, b.kv_lens, window=window, sinks=b.sinks if seed % 3 == 0 else None)
+    pool.check("prefill")
+    close(out, *b.want(window=window, sinks=seed % 3 == 0), dtype)
 
 
 def test_prefill_strided_q_layer_scale_and_stream(cuda):
@@ -391,7 +414,7 @@ def test_python_refusals(cuda):
         lambda: pool.decode(0, q, table, i32(5), out=q[:, :4]),
         lambda: pool.decode(0, q, table, i32(5), workspace=torch.zeros(8, device=cuda, dtype=torch.uint8)),
         lambda: pool.prefill(0, q, i32(0, 1, 1), table, i32(5)),
-        lambda: pool.prefill(0, q, i32(0, 1), table, i32(5), n_splits=65),
+        lambda: pool.prefill(0, q, i32(0, 1), table, i32(5), workspace=torch.zeros(8, device=cuda, dtype=torch.uint8)),
         lambda: pool.prefill(0, torch.zeros((1, 8, 132), dtype=BF, device=cuda)[:, :, :128], i32(0, 1), table, i32(5)),
         lambda: pool.append(0, kv, kv[:0], i32(1)),
         lambda: pool.append(0, kv, kv, i32(1, 2)),

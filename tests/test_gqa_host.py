@@ -24,9 +24,9 @@ def decode(v, layer=0, q=BASE, ts=1024, hs=128, n_seq=1, heads=8, pt=BASE, strid
 
 
 def prefill(v, layer=0, q=BASE, ts=1024, hs=128, n=1, heads=8, cu=BASE, n_seq=1, pt=BASE, stride=4, lens=BASE,
-            window=0, scale=0.1, splits=1, ws=BASE, out=BASE):
+            window=0, scale=0.1, ws=BASE, out=BASE):
     return _abi.load().rkv_gqa_prefill(addressof(v), layer, q, ts, hs, n, heads, cu, n_seq, pt, stride, lens, window,
-                                       0, scale, splits, ws, out, 0, 0)
+                                       0, scale, ws, out, 0, 0)
 
 
 def append(v, layer=0, k=BASE, ts=256, hs=128, vv=BASE, n=1, slots=BASE, rot=None, pos=BASE, q=0, heads=0, q_out=0):
@@ -45,9 +45,8 @@ def test_sizes():
     assert lib.rkv_gqa_page_bytes(0, 64) == lib.rkv_gqa_page_bytes(1, 96) == -1
     v = view(n_pages=1 << 16, n_layers=3, n_kv_heads=8)
     assert lib.rkv_gqa_bytes(addressof(v)) == 3 * (1 << 16) * 262144
-    assert lib.rkv_gqa_prefill_workspace_bytes(addressof(v), 100, 32, 1) == 0
-    assert lib.rkv_gqa_prefill_splits(addressof(v), 100000, 32, 4, 512) == 1
-    assert lib.rkv_gqa_prefill_splits(0, 1, 32, 4, 512) == lib.rkv_gqa_prefill_workspace_bytes(0, 1, 8, 1) == -1
+    assert lib.rkv_gqa_prefill_workspace_bytes(addressof(v)) >= 2 * 148 * 256 * (128 + 2) * 4
+    assert lib.rkv_gqa_prefill_workspace_bytes(0) == -1
     assert lib.rkv_gqa_decode_workspace_bytes(addressof(v), -1, 32) == -1
 
 
@@ -84,13 +83,14 @@ def test_attention_arguments(call):
 
 def test_decode_arguments():
     assert decode(view(), null=True) == ARG
+    assert decode(view(), ws=0) == ARG and decode(view(), ws=BASE + 8) == ARG
     assert decode(view(), n_seq=0, q=0, pt=0, lens=0, out=0, ws=0) == 0
 
 
 def test_prefill_arguments():
     v = view()
     assert prefill(v, n=-1) == SHAPE and prefill(v, cu=0) == ARG
-    assert prefill(v, splits=0) == SHAPE and prefill(v, splits=65) == SHAPE
+    assert prefill(v, ws=0) == ARG and prefill(v, ws=BASE + 8) == ARG
     assert prefill(v, n_seq=0) == SHAPE  # tokens without a sequence
     assert prefill(v, n=0, q=0, out=0) == 0
 
