@@ -480,13 +480,15 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) decode_kernel(const Para
 }
 
 // Joins the partial softmaxes of one (item, q head): first slot as recorded,
-// then slot 2 c of every later run c.  Warp w takes every eighth of them, lanes
-// the head's lanes; the eight sums are added in order.
-constexpr int kJoinWarps = 8;
+// then slot 2 c of every later run c.  A warp takes every sixteenth of them, four
+// at a time with their loads out together, lanes the head's lanes; the sixteen
+// sums are added in order.  (One long sequence of 2 kv heads has 148 parts an
+// item: 14 us with eight warps and one load after another.)
+constexpr int kJoinWarps = 16;
 template <typename T, int D>
 __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const Params p) {
   __shared__ float acc[kJoinWarps][D];
-  __shared__ float den[kJoinWarps];
+  __shared__ float2 ends[kJoinWarps];
   grid_dependency_wait();
   const int64_t item_id = blockIdx.x;
   const int hg = p.cache.n_kv_heads * p.chunks;
@@ -499,42 +501,55 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const Params p) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int count = span.y - span.x / 2 + 1;
   auto slot = [&](int i) { return (int64_t)(i == 0 ? span.x : 2 * (span.x / 2 + i)); };
-  const float sink = sink_log2(p.sinks, head);
-  float top = sink;
-  for (int i = lane; i < count; i += 32) top = fmaxf(top, p.part_ml[2 * (slot(i) * rows + r)]);
-#pragma unroll
-  for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-  if (top == -INFINITY) top = 0.f;
+  constexpr int kAhead = 4;
   float o[D / 32] = {};
-  float l = 0.f;
-#pragma unroll 4
-  for (int i = warp; i < count; i += kJoinWarps) {
-    const int64_t at = slot(i) * rows + r;
-    const float2 e = *reinterpret_cast<const float2*>(p.part_ml + 2 * at);
-    const float w = ex2(e.x - top);
-    l += w * e.y;
-    if constexpr (D == 128) {
-      const float4 v = *reinterpret_cast<const float4*>(p.part_o + at * D + 4 * lane);
-      o[0] += w * v.x;
-      o[1] += w * v.y;
-      o[2] += w * v.z;
-      o[3] += w * v.w;
-    } else {
-      const float2 v = *reinterpret_cast<const float2*>(p.part_o + at * D + 2 * lane);
-      o[0] += w * v.x;
-      o[1] += w * v.y;
+  float m = -INFINITY, l = 0.f;
+  for (int i0 = warp; i0 < count; i0 += kAhead * kJoinWarps) {
+    float2 e[kAhead];
+    float v[kAhead][D / 32];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int i = i0 + k * kJoinWarps;
+      e[k] = make_float2(-INFINITY, 0.f);
+      if (i >= count) continue;
+      const int64_t at = slot(i) * rows + r;
+      e[k] = *reinterpret_cast<const float2*>(p.part_ml + 2 * at);
+      if constexpr (D == 128) {
+        const float4 f = *reinterpret_cast<const float4*>(p.part_o + at * D + 4 * lane);
+        v[k][0] = f.x, v[k][1] = f.y, v[k][2] = f.z, v[k][3] = f.w;
+      } else {
+        const float2 f = *reinterpret_cast<const float2*>(p.part_o + at * D + 2 * lane);
+        v[k][0] = f.x, v[k][1] = f.y;
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      if (e[k].x == -INFINITY) continue;
+      const float top = fmaxf(m, e[k].x);
+      const float a = ex2(m - top), w = ex2(e[k].x - top);  // 0 from -inf
+      l = l * a + w * e[k].y;
+#pragma unroll
+      for (int j = 0; j < D / 32; ++j) o[j] = o[j] * a + w * v[k][j];
+      m = top;
     }
   }
 #pragma unroll
   for (int j = 0; j < D / 32; ++j) acc[warp][D / 32 * lane + j] = o[j];
-  if (lane == 0) den[warp] = l;
+  if (lane == 0) ends[warp] = make_float2(m, l);
   __syncthreads();
   if (threadIdx.x < D / 2) {
+    const float sink = sink_log2(p.sinks, head);
+    float top = sink;
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; ++w) top = fmaxf(top, ends[w].x);
+    if (top == -INFINITY) top = 0.f;
     float a = 0.f, b = 0.f, total = ex2(sink - top);
+#pragma unroll
     for (int w = 0; w < kJoinWarps; ++w) {
-      a += acc[w][2 * threadIdx.x];
-      b += acc[w][2 * threadIdx.x + 1];
-      total += den[w];
+      const float f = ex2(ends[w].x - top);
+      a += f * acc[w][2 * threadIdx.x];
+      b += f * acc[w][2 * threadIdx.x + 1];
+      total += f * ends[w].y;
     }
     const float inv = total == 0.f ? 0.f : 1.f / total;
     reinterpret_cast<uint32_t*>(p.out + (s * p.n_q_heads + head) * D)[threadIdx.x] = T::pack(a * inv, b * inv);

@@ -22,14 +22,13 @@
 // While a block ends, the next one's Q, K and V are copied and its first logits
 // computed.
 //
-//   warps 0-15      softmax, one row a thread: S from tensor memory, running
-//                   maximum and sum, P (in the cache's type) back over S; the
-//                   epilogue.  Four warps have the even steps of tile 0, four
-//                   its odd steps, and so for tile 1
-//   warps 16, 17    issue S = Q K^T (Q, K in shared memory) and O += P V (P in
+//   warps 0-3, 4-7  softmax of tile 0 and of tile 1, one row a thread: S from
+//                   tensor memory, running maximum and sum, P (in the cache's
+//                   type) back over S; the epilogue
+//   warps 8, 9      issue S = Q K^T (Q, K in shared memory) and O += P V (P in
 //                   tensor memory, V in shared memory) of tile 0 and of tile 1
-//   warp 18         copies Q, K and V by tensor maps into a ring of stages
-//   warp 19         walks the run and hands out its blocks
+//   warp 10         copies Q, K and V by tensor maps into a ring of stages
+//   warp 11         walks the run and hands out its blocks
 //
 // Tensor memory: two S buffers of 64 columns for each tile (P over the first 32
 // of its own), O0, O1 (head_dim columns each).  S of step j + 2 is issued behind
@@ -41,12 +40,20 @@
 // issued, so each tile has a warp of its own for it: one warp for both left
 // them idle for the 200-700 clocks of its waits between two batches.
 //
-// The exponentials of a step take four warps (one a scheduler) 512 clocks at the
-// least; the loads, maxima, conversions and waits around them as long again.  So
-// two sets of warps take a tile's steps in turn, one's latencies behind the
-// other's exponentials.  They share the rows' exponent reference: a step's
-// warps publish it (shared memory, one barrier a warp) as soon as they have
-// their maxima, and the next step's take it from there.
+// What bounds a step of both tiles (1650 to 1750 clocks, head_dim 128): 1280 of
+// MMAs -- S with 64 columns reads 6 KB of operands for 32 clocks of products, the
+// shared memory's 128 bytes a clock make it 48 -- and a chain of the softmax
+// warps: 290 for loads, maxima and masks, 930 for 64 exponentials, conversions
+// and sums (1070 when both tiles' warps meet there; 512 each at 16 a clock), and
+// 150 to 250 for every barrier while the operand reads fill the shared memory.
+// Measured and not kept: two sets of softmax warps taking a tile's steps in
+// turn (head_dim 128: 539 us instead of 527 for 8192 tokens; head_dim 64: 5%
+// faster); the tiles' warps handing each other the exponentials by named barriers
+// (550); a cubic on the FMA pipe for a quarter of the exponentials (+2%, for half
+// of them +12%); other orders of the same instructions (no change).
+//
+// 8192 tokens, 32 q and 8 kv heads of 128, bf16: 527 us, 1.04 PFLOP/s, with the
+// clock at 1.7 GHz under the power limit; 445 us for a single pass.
 #include <atomic>
 
 #include "rkv_gqa.cuh"
@@ -57,19 +64,19 @@ namespace pre {
 
 constexpr int kM = 128;        // q rows of a tile
 constexpr int kN = kPage;      // key rows of a step
-constexpr int kThreads = 640;
-constexpr int kMmaWarp = 16, kLoadWarp = 18, kPlanWarp = 19;
+constexpr int kMmaWarp = 8, kLoadWarp = 10, kPlanWarp = 11;
+constexpr int kThreads = 384;
 constexpr int kGrid = 148;         // one CTA an SM
 constexpr int kBlockRows = 2 * kM;
 constexpr int kBlockCost = 192;    // what a block costs beside its rows, in rows
 constexpr int kRunCost = 8 * kN + kBlockCost;  // no more CTAs than have this much, or a block each
 constexpr int kJobs = 4;           // blocks handed out ahead
 constexpr uint32_t kTmemCols = 512;
-// The launch has 96 registers a thread; the four softmax warpgroups take what the
-// fifth does without.  (Calls that are not inlined do not go with it: ptxas
+// The launch has 168 registers a thread; the two softmax warpgroups take what the
+// third does without.  (Calls that are not inlined do not go with it: ptxas
 // does not end.)
-constexpr int kSoftmaxRegs = 104, kOtherRegs = 64;
-static_assert(4 * kSoftmaxRegs + kOtherRegs <= 5 * 96, "more registers than the launch has");
+constexpr int kSoftmaxRegs = 192, kOtherRegs = 120;
+static_assert(2 * kSoftmaxRegs + kOtherRegs <= 3 * 168, "more registers than the launch has");
 
 struct Params {
   rkv_gqa_view cache;
@@ -94,13 +101,11 @@ template <int D>
 struct Layout {
   static constexpr int kQ = kM * D * 2;      // bytes of a Q tile
   static constexpr int kStage = kN * D * 2;  // K or V of a page
-  static constexpr int kStages = D == 128 ? 9 : 16;
+  static constexpr int kStages = D == 128 ? 10 : 16;
   static constexpr int kQCol = kM * 128;     // a 64-lane column block of a Q tile
   static constexpr int kCol = kN * 128;      // and of a page
   static constexpr int kRing = 2 * kQ;
-  static constexpr int kEnds = kRing + kStages * kStage;  // [2][2 tiles][2 sets][128] reference and sum at a block's end
-  static constexpr int kRef = kEnds + 8192;               // exponent references [2][128]
-  static constexpr int kJob = kRef + 1024;                // [kJobs] of 64 bytes
+  static constexpr int kJob = kRing + kStages * kStage;   // [kJobs] of 64 bytes
   static constexpr int kBars = kJob + 64 * kJobs;
   static constexpr int kBarEmpty = 8 * kStages;   // full[kStages], empty[kStages]
   static constexpr int kBarS = 16 * kStages;      // S full [2][2]
@@ -108,14 +113,12 @@ struct Layout {
   static constexpr int kBarPv = kBarP + 32;       // O += P V of a step done [2]
   static constexpr int kBarO = kBarPv + 16;       // O of a block done [2]
   static constexpr int kBarOFree = kBarO + 16;    // and read [2]
-  static constexpr int kBarEnds = kBarOFree + 16; // both sets' ends written [2]
-  static constexpr int kBarRef = kBarEnds + 16;   // reference of a step written [2][4]
-  static constexpr int kBarQ = kBarRef + 64;      // Q full, Q free
+  static constexpr int kBarQ = kBarOFree + 16;    // Q full, Q free
   static constexpr int kBarJob = kBarQ + 16;      // job full[kJobs], free[kJobs]
   static constexpr int kBarDrain = kBarJob + 16 * kJobs;  // [2]
   static constexpr int kMisc = kBars + kBarDrain + 16;    // TMEM address, abort flag, start of the run
-  static constexpr int kScan = kMisc + 32;                // [20] sums of the warps: costs, blocks
-  static constexpr int kTotal = kScan + 12 * 20 + 1024;   // slack for the 1024-byte alignment
+  static constexpr int kScan = kMisc + 32;                // sums of the warps: costs, blocks
+  static constexpr int kTotal = kScan + 12 * (kThreads / 32) + 1024;  // slack for the 1024-byte alignment
 };
 
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -289,7 +292,7 @@ prefill_kernel(const Params p, const __grid_constant__ CUtensorMap map, const __
   volatile int* start_seq = reinterpret_cast<volatile int*>(smem + L::kMisc + 8);
   volatile long long* start_off = reinterpret_cast<volatile long long*>(smem + L::kMisc + 16);
   long long* scan = reinterpret_cast<long long*>(smem + L::kScan);
-  int* block_sums = reinterpret_cast<int*>(smem + L::kScan + 160);
+  int* block_sums = reinterpret_cast<int*>(smem + L::kScan + 8 * (kThreads / 32));
 
   if (tid == 0) {
     for (int i = 0; i < L::kStages; ++i) {
@@ -303,11 +306,9 @@ prefill_kernel(const Params p, const __grid_constant__ CUtensorMap map, const __
     for (int t = 0; t < 2; ++t) {
       mbar_init(bars + L::kBarPv + 8 * t, 1);
       mbar_init(bars + L::kBarO + 8 * t, 1);
-      mbar_init(bars + L::kBarOFree + 8 * t, 8);  // warps of a tile
-      mbar_init(bars + L::kBarEnds + 8 * t, 8);
+      mbar_init(bars + L::kBarOFree + 8 * t, 4);  // warps of a tile
       mbar_init(bars + L::kBarDrain + 8 * t, 1);
     }
-    for (int i = 0; i < 8; ++i) mbar_init(bars + L::kBarRef + 8 * i, 1);
     mbar_init(bars + L::kBarQ, 1);
     mbar_init(bars + L::kBarQ + 8, 2);
     for (int i = 0; i < kJobs; ++i) {
@@ -678,14 +679,12 @@ prefill_kernel(const Params p, const __grid_constant__ CUtensorMap map, const __
   } else {
     // --------------------------------------------------------------- softmax
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
-    const int t = warp >> 3, b = (warp >> 2) & 1;       // tile, and which of its S buffers (and so steps)
+    const int t = warp >> 2;                            // tile
     const int r = 32 * (warp & 3) + lane;               // row of the tile
     const int row_token = t * p.tile_tokens + r / p.group;  // of a job's tokens
     const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
-    const uint32_t ts = tmem + lanes + t * 128 + 64 * b;
+    const uint32_t ts0 = tmem + lanes + t * 128;
     const uint32_t to = tmem + lanes + 256 + t * D;
-    const uint32_t ref_bar = bars + L::kBarRef + 32 * t + 8 * (warp & 3);
-    volatile float* ref = reinterpret_cast<volatile float*>(smem + L::kRef) + 128 * t + r;
     const unsigned long long c2 = dup2(p.scale_log2);
     int n = 0;    // steps of this tile so far: of step j of a job, n + j
     int n_o = 0;  // jobs in which the tile had some
@@ -707,9 +706,12 @@ prefill_kernel(const Params p, const __grid_constant__ CUtensorMap map, const __
       const int pos_min = t * p.tile_tokens;                       // the tile's first and last position from there
       const int pos_max = pos_min + p.tile_tokens - 1;
       float m = -INFINITY;  // exponent reference of l
-      float l = 0.f;        // sum of the weights of this set's steps
-      for (int j = (n ^ b) & 1; j < steps; j += 2) {
-        if (!__all_sync(0xffffffffu, mbar_wait(bars + L::kBarS + 16 * t + 8 * b, ((n + j) >> 1) & 1, abort_flag))) {
+      float l = 0.f;        // sum of the weights
+      bool ready = false;
+      for (int j = 0; j < steps; ++j) {
+        const int b = (n + j) & 1;
+        const uint32_t ts = ts0 + 64 * b;
+        if (!__all_sync(0xffffffffu, ready || mbar_wait(bars + L::kBarS + 16 * t + 8 * b, ((n + j) >> 1) & 1, abort_flag))) {
           ok = false;
           break;
         }
@@ -737,25 +739,12 @@ prefill_kernel(const Params p, const __grid_constant__ CUtensorMap map, const __
         t0 = fmax3(t0, __uint_as_float(x[kN - 4]), __uint_as_float(x[kN - 3]));
         t1 = fmax3(t1, __uint_as_float(x[kN - 2]), __uint_as_float(x[kN - 1]));
         const float top = fmaxf(fmax3(t0, t1, t2), t3) * p.scale_log2 - SoftmaxBias<T>::kBias;
-        // the reference that the step before left, and this step's
-        float was = m;
-        if (j > 0) {
-          if (!__all_sync(0xffffffffu, mbar_wait(ref_bar, (n + j - 1) & 1, abort_flag))) {
-            ok = false;
-            break;
-          }
-          was = *ref;
-        }
-        const bool up = top > was + kLazyLog2 || (was == -INFINITY && top > -INFINITY);
-        const float now = up ? top : was;
-        *ref = now;
-        __syncwarp();
-        if (lane == 0) mbar_arrive(ref_bar);
-        if (__any_sync(0xffffffffu, now != m)) {  // it moved in this step or in the one before
-          l *= now == m ? 1.f : ex2(m - now);     // 0 from -inf
-          m = now;
-          if (j > 0 && __any_sync(0xffffffffu, up)) {
-            const float a = up ? ex2(was - now) : 1.f;
+        const bool up = top > m + kLazyLog2 || (m == -INFINITY && top > -INFINITY);
+        if (__any_sync(0xffffffffu, up)) {
+          const float a = up ? ex2(m - top) : 1.f;  // 0 from -inf
+          m = up ? top : m;
+          l *= a;
+          if (j > 0) {
             // O holds the steps up to j - 1 once their MMAs are done: S of this step was issued behind step j - 2's,
             // and step j's wait for this warp, so the barrier is in that phase or just past it
             if (!__all_sync(0xffffffffu, mbar_wait(bars + L::kBarPv + 8 * t, (n + j - 1) & 1, abort_flag))) {
@@ -774,6 +763,10 @@ prefill_kernel(const Params p, const __grid_constant__ CUtensorMap map, const __
             }
           }
         }
+        // Asked here, the next S's barrier answers behind the exponentials.  With head_dim 64 that is 4% (360 to 345
+        // us for 8 x 64-256 tokens behind 8192 rows); with 128, S is not there yet and it costs 2%.
+        if constexpr (D == 64)
+          ready = j + 1 < steps && mbar_test(bars + L::kBarS + 16 * t + 8 * (1 - b), ((n + j + 1) >> 1) & 1);
         const unsigned long long n2 = dup2(m == -INFINITY ? 0.f : -m);  // nothing seen yet: weights 0
         l += weights<T>(x, ts, c2, n2);
         tmem_wait_st();
@@ -781,19 +774,10 @@ prefill_kernel(const Params p, const __grid_constant__ CUtensorMap map, const __
         mbar_arrive(bars + L::kBarP + 16 * t + 8 * b);
       }
       if (!ok) break;
-      // ---- epilogue: both sets' sums together, then one row a thread, half of its lanes a set
+      // ---- epilogue: one row a thread
       if (steps > 0) {
-        float2* ends = reinterpret_cast<float2*>(smem + L::kEnds) + 512 * (n_o & 1) + 256 * t + r;
-        ends[128 * b] = make_float2(m, l);
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bars + L::kBarEnds + 8 * t);
-        ok = __all_sync(0xffffffffu, mbar_wait(bars + L::kBarEnds + 8 * t, n_o & 1, abort_flag)) &&
-             __all_sync(0xffffffffu, mbar_wait(bars + L::kBarO + 8 * t, n_o & 1, abort_flag));
+        ok = __all_sync(0xffffffffu, mbar_wait(bars + L::kBarO + 8 * t, n_o & 1, abort_flag));
         if (!ok) break;
-        const float2 other = ends[128 * (1 - b)];
-        const float mm = fmaxf(m, other.x);
-        if (mm != -INFINITY) l = l * ex2(m - mm) + other.y * ex2(other.x - mm);
-        m = mm;
         tc_fence_after();
         n += steps;
         n_o += 1;
@@ -811,7 +795,7 @@ prefill_kernel(const Params p, const __grid_constant__ CUtensorMap map, const __
       float f = seen ? 1.f : 0.f;
       const int64_t at = (int64_t)w.slot * kBlockRows + t * kM + row;
       if (w.slot >= 0) {
-        if (live && b == 0) *reinterpret_cast<float2*>(p.part_ml + 2 * at) = make_float2(m, l);
+        if (live) *reinterpret_cast<float2*>(p.part_ml + 2 * at) = make_float2(m, l);
       } else if (live && seen) {
         const float sink = p.sinks ? p.sinks[head] * 1.4426950408889634f : -INFINITY;
         const float top = fmaxf(m, sink);
@@ -820,12 +804,12 @@ prefill_kernel(const Params p, const __grid_constant__ CUtensorMap map, const __
       }
       uint16_t* dst = p.out + ((int64_t)(w.token + token) * p.n_q_heads + head) * D;
 #pragma unroll 1
-      for (int c = b * (D / 2); c < (b + 1) * (D / 2); c += 32) {
+      for (int c = 0; c < D; c += 32) {
         uint32_t o[32];
         if (steps > 0) {
           tmem_ld32(to + c, o);
           tmem_wait_ld();
-          if (c + 32 == (b + 1) * (D / 2)) {  // O may be overwritten
+          if (c + 32 == D) {  // O may be overwritten
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(bars + L::kBarOFree + 8 * t);
@@ -866,43 +850,89 @@ prefill_kernel(const Params p, const __grid_constant__ CUtensorMap map, const __
 
 // Joins the parts of the block whose first part is the end of run c, in the
 // order of their rows: slot 2 c + 1, then slot 2 c' of the runs after it up to the
-// block's last part.  A warp a row, 32 rows a CTA.
+// block's last part.  32 rows a CTA, four a warp, whose loads go out together.
+constexpr int kJoinThreads = 256;
 template <typename T, int D>
-__global__ void __launch_bounds__(256) join_kernel(const Params p) {
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p) {
+  __shared__ int slots[kGrid];
+  __shared__ int counts[kJoinThreads / 32];
+  __shared__ int ends[kJoinThreads / 32];
   grid_dependency_wait();
-  const int c = blockIdx.x;
+  const int c = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int4 block = p.parts[2 * c + 1];
-  if (block.w == 0) return;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int i = warp; i < 32; i += 8) {
-    const int row = blockIdx.y * 32 + i, t = row / kM, r = row % kM;
-    const int token = t * p.tile_tokens + r / p.group;
-    if (r >= p.tile_tokens * p.group || token >= block.y) continue;
-    const int head = block.z * p.group + r % p.group;
-    const float sink = p.sinks ? p.sinks[head] * 1.4426950408889634f : -INFINITY;
-    float m = sink, l = sink == -INFINITY ? 0.f : 1.f;
-    float o[D / 32] = {};
-    for (int from = c; from < kGrid; ++from) {
-      const int slot = from == c ? 2 * c + 1 : 2 * from;
-      const int4 part = p.parts[slot];
-      // a run whose share of the block was cut away has none
-      if (part.w == 0 || part.x != block.x || part.z != block.z) continue;
-      const int64_t at = (int64_t)slot * kBlockRows + row;
-      const float2 e = *reinterpret_cast<const float2*>(p.part_ml + 2 * at);
-      if (e.x != -INFINITY) {
-        const float top = fmaxf(m, e.x);
-        const float a = ex2(m - top), w = ex2(e.x - top);  // 0 from -inf
-        l = l * a + e.y * w;
+  if (block.w == 0 || (blockIdx.y * 32 >= kM && block.y <= p.tile_tokens)) return;
+  // the list of slots: thread i looks at run c + 1 + i; those past the block's last part do not count
+  const int from = c + 1 + threadIdx.x;
+  int4 part = make_int4(0, 0, 0, 0);
+  if (from < kGrid) part = p.parts[2 * from];
+  const bool mine = part.w != 0 && part.x == block.x && part.z == block.z;  // a run whose share was cut away has none
+  const unsigned has = __ballot_sync(0xffffffffu, mine), last = __ballot_sync(0xffffffffu, mine && part.w == 3);
+  const unsigned upto = last ? (last & (0u - last)) | ((last & (0u - last)) - 1u) : 0xffffffffu;  // up to the first last part
+  if (lane == 0) {
+    counts[warp] = __popc(has & upto);
+    ends[warp] = last != 0u;
+  }
+  __syncthreads();
+  int before = 1, n = 1;
+  bool ended = false;
+  for (int i = 0; i < kJoinThreads / 32; ++i) {
+    if (i == warp && ended) before = -1;
+    if (i < warp && before > 0) before += counts[i];
+    if (!ended) n += counts[i];
+    ended = ended || ends[i];
+  }
+  if (before > 0 && mine && ((upto >> lane) & 1u)) slots[before + __popc(has & ((1u << lane) - 1u))] = 2 * from;
+  if (threadIdx.x == 0) slots[0] = 2 * c + 1;
+  __syncthreads();
+
+  constexpr int kMine = 4;
+  int row[kMine];
+  float m[kMine], l[kMine], o[kMine][D / 32];
 #pragma unroll
-        for (int j = 0; j < D / 32; ++j) o[j] = o[j] * a + w * p.part_o[at * D + D / 32 * lane + j];
-        m = top;
+  for (int k = 0; k < kMine; ++k) {
+    row[k] = blockIdx.y * 32 + warp + 8 * k;
+    const int head = block.z * p.group + row[k] % kM % p.group;
+    m[k] = p.sinks ? p.sinks[head] * 1.4426950408889634f : -INFINITY;
+    l[k] = m[k] == -INFINITY ? 0.f : 1.f;
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j) o[k][j] = 0.f;
+  }
+  for (int i = 0; i < n; ++i) {
+    const int64_t at = (int64_t)slots[i] * kBlockRows;
+    float2 e[kMine];
+    float v[kMine][D / 32];
+#pragma unroll
+    for (int k = 0; k < kMine; ++k) {
+      e[k] = *reinterpret_cast<const float2*>(p.part_ml + 2 * (at + row[k]));
+      const float* src = p.part_o + (at + row[k]) * D + D / 32 * lane;
+      if constexpr (D == 128) {
+        const float4 f = *reinterpret_cast<const float4*>(src);
+        v[k][0] = f.x, v[k][1] = f.y, v[k][2] = f.z, v[k][3] = f.w;
+      } else {
+        const float2 f = *reinterpret_cast<const float2*>(src);
+        v[k][0] = f.x, v[k][1] = f.y;
       }
-      if (part.w == 3) break;
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+    for (int k = 0; k < kMine; ++k) {
+      if (e[k].x == -INFINITY) continue;  // it saw nothing there, and wrote no O
+      const float top = fmaxf(m[k], e[k].x);
+      const float a = ex2(m[k] - top), w = ex2(e[k].x - top);  // 0 from -inf
+      l[k] = l[k] * a + e[k].y * w;
+#pragma unroll
+      for (int j = 0; j < D / 32; ++j) o[k][j] = o[k][j] * a + w * v[k][j];
+      m[k] = top;
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < kMine; ++k) {
+    const int r = row[k] % kM, token = row[k] / kM * p.tile_tokens + r / p.group;
+    if (r >= p.tile_tokens * p.group || token >= block.y) continue;
+    const float inv = l[k] == 0.f ? 0.f : 1.f / l[k];
+    const int head = block.z * p.group + r % p.group;
     uint32_t* dst = reinterpret_cast<uint32_t*>(p.out + ((int64_t)(block.x + token) * p.n_q_heads + head) * D) + D / 64 * lane;
 #pragma unroll
-    for (int j = 0; j < D / 64; ++j) dst[j] = T::pack(o[2 * j] * inv, o[2 * j + 1] * inv);
+    for (int j = 0; j < D / 64; ++j) dst[j] = T::pack(o[k][2 * j] * inv, o[k][2 * j + 1] * inv);
   }
 }
 
@@ -931,7 +961,7 @@ static rkv_status launch(const Params& p, const CUtensorMap& map, const CUtensor
   cudaError_t e = cudaLaunchKernelEx(&cfg, prefill_kernel<T, D>, p, map, qmap);
   if (e == cudaSuccess) {
     cfg.gridDim = dim3(kGrid, kBlockRows / 32);
-    cfg.blockDim = dim3(256);
+    cfg.blockDim = dim3(kJoinThreads);
     cfg.dynamicSmemBytes = 0;
     e = cudaLaunchKernelEx(&cfg, join_kernel<T, D>, p);
   }
