@@ -120,111 +120,156 @@ struct AppendParams {
   uint32_t* status;
 };
 
-// One CTA per token.  A work item is 16 lanes of one head's row: with
-// rotation, the 8 + 8 lanes that eight pairs need (two 16-byte chunks half a
-// rotary width apart, or 16 lanes in a row when interleaved), else 16 lanes in
-// a row.  Items of q come first, then k, then v.
-template <typename T, bool kInterleaved>
-__global__ void __launch_bounds__(128) append_kernel(const AppendParams p) {
-  const int64_t t = blockIdx.x;
-  const int d = p.cache.head_dim, per_row = d / 16, hkv = p.cache.n_kv_heads;
-  const int slot = p.slots[t];
-  bool store = slot >= 0, bad_pos = false;
-  if (store && slot >= p.cache.n_pages * kPage) {
-    store = false;
-    if (threadIdx.x == 0) set_status(p.status, RKV_ERR_INDEX_OUT_OF_RANGE);
+// A CTA takes one token after another, and of each kHeads heads (blockIdx.y says
+// which; those of q come first, then k, then v).  A thread has the 16 lanes of chunk
+// c of kAhead heads: with rotation, the 8 + 8 lanes that eight pairs need (two
+// 16-byte chunks half a rotary width apart, or 16 lanes in a row when
+// interleaved), else 16 lanes in a row; so it loads its eight cosines and sines once
+// for all of them, and what depends on its heads it works out once for all tokens.
+//
+// Bytes bound it -- every row once in and once out -- if the instructions are few
+// and the bytes on their way many: a token's slot and positions are loaded while
+// the one before is worked on, so that its rows and its cosines and sines are
+// one trip to memory together.
+constexpr int kAppendThreads = 128, kAhead = 3, kAppendCtas = 6;
+template <int D>
+struct AppendShape {
+  static constexpr int kPerRow = D / 16;                    // threads of a row: lanes of one warp
+  static constexpr int kStep = kAppendThreads / kPerRow;    // heads at a time
+  static constexpr int kHeads = kAhead * kStep;             // heads of a CTA: 48 (head_dim 128) or 96
+};
+template <typename T, int D, bool kInterleaved>
+__global__ void __launch_bounds__(kAppendThreads, kAppendCtas) append_kernel(const AppendParams p) {
+  using A = AppendShape<D>;
+  const int c = threadIdx.x % A::kPerRow, hkv = p.cache.n_kv_heads, heads = p.n_q_heads + 2 * hkv;
+  const int half = p.rot / 2;
+  // ---- per thread: where its chunk lies, and its heads
+  const bool turned = 16 * c < p.rot;  // rotated in q and k
+  const int a1 = turned && !kInterleaved ? 8 * c : 16 * c, b1 = turned && !kInterleaved ? a1 + half : a1 + 8;
+  const int axes = p.rot ? 1 + (p.edge[0] < half) + (p.edge[1] < half) + (p.edge[2] < half) : 0;
+  auto axis_of = [&](int pair) { return (pair >= p.edge[0]) + (pair >= p.edge[1]) + (pair >= p.edge[2]); };
+  const int axis0 = axis_of(8 * c), axis7 = axis_of(8 * c + 7);  // mostly the same
+  const float2* const table = reinterpret_cast<const float2*>(p.table) + 8 * c;
+  enum { kQ, kK, kV, kNone };
+  int kind[kAhead];
+  const uint16_t* src[kAhead];  // of token 0
+  int64_t src_ts[kAhead];
+  int64_t dst_at[kAhead];       // elements from the token's row in q_out, or from its page and row in the cache
+#pragma unroll
+  for (int k = 0; k < kAhead; ++k) {
+    const int h = blockIdx.y * A::kHeads + k * A::kStep + threadIdx.x / A::kPerRow;
+    kind[k] = h < p.n_q_heads ? kQ : h < p.n_q_heads + hkv ? kK : h < heads ? kV : kNone;
+    const int head = kind[k] == kQ ? h : kind[k] == kK ? h - p.n_q_heads : h - p.n_q_heads - hkv;
+    src[k] = kind[k] == kQ ? p.q + head * p.q_hs : kind[k] == kK ? p.k + head * p.k_hs : p.v + head * p.v_hs;
+    src_ts[k] = kind[k] == kQ ? p.q_ts : kind[k] == kK ? p.k_ts : p.v_ts;
+    dst_at[k] = kind[k] == kQ ? (int64_t)head * D : (int64_t)((kind[k] == kV ? hkv : 0) + head) * kPage * D;
   }
-  int32_t pos[4] = {0, 0, 0, 0};
-  if (p.rot) {
-    const int axes = 1 + (p.edge[0] < p.rot / 2) + (p.edge[1] < p.rot / 2) + (p.edge[2] < p.rot / 2);
+  const int64_t page_elems = (int64_t)2 * hkv * kPage * D;
+  uint16_t* const layer_base = static_cast<uint16_t*>(p.cache.base) + p.layer * p.cache.n_pages * page_elems;
+
+  int slot = 0, pos[4] = {0, 0, 0, 0};
+  auto look = [&](int64_t t) {
+    if (t >= p.n_tokens) return;
+    slot = p.slots[t];
 #pragma unroll
     for (int a = 0; a < 4; ++a)
-      if (a < axes) {
-        pos[a] = p.pos[(int64_t)a * p.n_tokens + t];
-        bad_pos |= pos[a] < 0 || pos[a] >= p.table_rows;
-      }
+      if (a < axes) pos[a] = p.pos[(int64_t)a * p.n_tokens + t];
+  };
+  look(blockIdx.x);
+  for (int64_t t = blockIdx.x; t < p.n_tokens; t += gridDim.x) {
+    bool store = slot >= 0, bad_pos = false;
+    if (store && slot >= p.cache.n_pages * kPage) {
+      store = false;
+      if (threadIdx.x == 0) set_status(p.status, RKV_ERR_INDEX_OUT_OF_RANGE);
+    }
+#pragma unroll
+    for (int a = 0; a < 4; ++a) bad_pos |= a < axes && (pos[a] < 0 || pos[a] >= p.table_rows);
     if (bad_pos) {
       store = false;
       if (threadIdx.x == 0) set_status(p.status, RKV_ERR_INDEX_OUT_OF_RANGE);
     }
-  }
-  const int64_t page = store ? slot / kPage : 0;
-  const int row = store ? slot % kPage : 0;
-  const int heads = p.n_q_heads + 2 * hkv;
-  // the items of a row are 4 or 8 consecutive lanes of one warp
-  for (int item = threadIdx.x; item < (heads * per_row + 31) / 32 * 32; item += blockDim.x) {
-    const int h = item / per_row, c = item % per_row;
-    const bool live = h < heads;
-    const bool is_q = h < p.n_q_heads, is_v = h >= p.n_q_heads + hkv;
-    const int head = is_q ? h : is_v ? h - p.n_q_heads - hkv : h - p.n_q_heads;
-    const uint16_t* src = is_q ? p.q + t * p.q_ts + head * p.q_hs
-                          : is_v ? p.v + t * p.v_ts + head * p.v_hs
-                                 : p.k + t * p.k_ts + head * p.k_hs;
-    // first lanes of the two chunks
-    const bool turn = p.rot > 0 && !is_v && 16 * c < p.rot;
-    const int a = turn && !kInterleaved ? 8 * c : 16 * c;
-    const int b = turn && !kInterleaved ? a + p.rot / 2 : a + 8;
-    uint32_t x[4] = {0, 0, 0, 0}, y[4] = {0, 0, 0, 0};
-    const bool read = live && (is_q || store);
-    if (read) {
-      *reinterpret_cast<uint4*>(x) = *reinterpret_cast<const uint4*>(src + a);
-      *reinterpret_cast<uint4*>(y) = *reinterpret_cast<const uint4*>(src + b);
-    }
-    if (read && turn && !bad_pos) {
-      float2 u[4], w[4];  // the pairs' first and second members, two pairs an entry
+    uint16_t* const row = layer_base + (slot / kPage) * page_elems + slot % kPage * D;  // used if stored
+    uint16_t* const q_row = p.q_out + t * p.n_q_heads * D;
+    uint4 u[kAhead], w[kAhead];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (kInterleaved) {  // word i of x is pair i, word i of y pair 4 + i
+    for (int k = 0; k < kAhead; ++k) {
+      u[k] = w[k] = make_uint4(0, 0, 0, 0);
+      if (kind[k] == kNone || !(kind[k] == kQ || store)) continue;
+      const uint16_t* at = src[k] + t * src_ts[k];
+      u[k] = *reinterpret_cast<const uint4*>(at + (kind[k] == kV ? 16 * c : a1));
+      w[k] = *reinterpret_cast<const uint4*>(at + (kind[k] == kV ? 16 * c + 8 : b1));
+    }
+    float2 cs[8];  // cosine and sine of pairs 8 c ..
+    if (turned && !bad_pos) {
+      auto pos_of = [&](int axis) { return axis == 0 ? pos[0] : axis == 1 ? pos[1] : axis == 2 ? pos[2] : pos[3]; };
+      if (axis0 == axis7) {
+        const float4* from = reinterpret_cast<const float4*>(table + (int64_t)pos_of(axis0) * half);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float4 f = __ldg(from + i);
+          cs[2 * i] = make_float2(f.x, f.y);
+          cs[2 * i + 1] = make_float2(f.z, f.w);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) cs[i] = __ldg(table + (int64_t)pos_of(axis_of(8 * c + i)) * half + i);
+      }
+    }
+    look(t + gridDim.x);
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      uint32_t x[4] = {u[k].x, u[k].y, u[k].z, u[k].w}, y[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
+      if (turned && !bad_pos && kind[k] < kV) {
+        // interleaved: word i of x is pair i, word i of y pair 4 + i; else x holds the pairs' first members, y the second
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
           const float2 e = T::unpack(x[i]), f = T::unpack(y[i]);
-          u[i] = make_float2(e.x, f.x);
-          w[i] = make_float2(e.y, f.y);
-        } else {
-          u[i] = T::unpack(x[i]);
-          w[i] = T::unpack(y[i]);
+          const float2 c0 = cs[kInterleaved ? i : 2 * i], c1 = cs[kInterleaved ? 4 + i : 2 * i + 1];
+          const float u0 = e.x, w0 = kInterleaved ? e.y : f.x, u1 = kInterleaved ? f.x : e.y, w1 = f.y;
+          const float r0 = u0 * c0.x - w0 * c0.y, s0 = w0 * c0.x + u0 * c0.y;
+          const float r1 = u1 * c1.x - w1 * c1.y, s1 = w1 * c1.x + u1 * c1.y;
+          x[i] = kInterleaved ? T::pack(r0, s0) : T::pack(r0, r1);
+          y[i] = kInterleaved ? T::pack(r1, s1) : T::pack(s0, s1);
         }
       }
-      float2 ru[4], rw[4];
+      // a K or V row is refused as a whole: its threads vote
+      const bool cached = kind[k] == kK || kind[k] == kV;
+      bool bad = false;
+      if (cached) {
+        uint32_t top = 0;  // largest magnitude bits
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int p0 = 8 * c + (kInterleaved ? i : 2 * i), p1 = 8 * c + (kInterleaved ? 4 + i : 2 * i + 1);
-        auto cs = [&](int pair) {
-          const int axis = (pair >= p.edge[0]) + (pair >= p.edge[1]) + (pair >= p.edge[2]);
-          const int32_t at = axis == 0 ? pos[0] : axis == 1 ? pos[1] : axis == 2 ? pos[2] : pos[3];
-          return __ldg(reinterpret_cast<const float2*>(p.table) + (int64_t)at * (p.rot / 2) + pair);
-        };
-        const float2 c0 = cs(p0), c1 = cs(p1);
-        ru[i] = make_float2(u[i].x * c0.x - w[i].x * c0.y, u[i].y * c1.x - w[i].y * c1.y);
-        rw[i] = make_float2(w[i].x * c0.x + u[i].x * c0.y, w[i].y * c1.x + u[i].y * c1.y);
+        for (int i = 0; i < 4; ++i) top = __vmaxu2(top, __vmaxu2(x[i] & 0x7fff7fffu, y[i] & 0x7fff7fffu));
+        bad = store && max(top & 0xffffu, top >> 16) >= T::kExpMask;
       }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        x[i] = kInterleaved ? T::pack(ru[i].x, rw[i].x) : T::pack(ru[i].x, ru[i].y);
-        y[i] = kInterleaved ? T::pack(ru[i].y, rw[i].y) : T::pack(rw[i].x, rw[i].y);
-      }
-    }
-    // a K or V row is refused as a whole: its lanes vote
-    bool bad = false;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) bad |= not_finite<T>(x[i]) || not_finite<T>(y[i]);
-    const unsigned votes = __ballot_sync(0xffffffffu, bad && read && !is_q);
-    const int first = (threadIdx.x & 31) / per_row * per_row;
-    const bool refused = ((votes >> first) & ((1u << per_row) - 1u)) != 0u;
-    uint16_t* dst;
-    bool write = live;
-    if (is_q) {
-      dst = p.q_out + (t * p.n_q_heads + head) * d;
-      if (bad_pos)
+      const unsigned votes = __ballot_sync(0xffffffffu, bad);
+      const bool refused = ((votes >> ((threadIdx.x & 31) / A::kPerRow * A::kPerRow)) & ((1u << A::kPerRow) - 1u)) != 0u;
+      if (kind[k] == kNone) continue;
+      if (cached) {
+        if (refused) set_status(p.status, RKV_ERR_NON_FINITE_INPUT);
+        if (!store || refused) continue;
+      } else if (bad_pos) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) x[i] = y[i] = 0u;
-    } else {
-      dst = static_cast<uint16_t*>(p.cache.base) + (row_base(p.cache, p.layer, page, is_v, live ? head : 0) + row) * d;
-      write = live && store && !refused;
-      if (refused && live) set_status(p.status, RKV_ERR_NON_FINITE_INPUT);
+      }
+      uint16_t* dst = (cached ? row : q_row) + dst_at[k];
+      *reinterpret_cast<uint4*>(dst + (kind[k] == kV ? 16 * c : a1)) = make_uint4(x[0], x[1], x[2], x[3]);
+      *reinterpret_cast<uint4*>(dst + (kind[k] == kV ? 16 * c + 8 : b1)) = make_uint4(y[0], y[1], y[2], y[3]);
     }
-    if (write) {
-      *reinterpret_cast<uint4*>(dst + a) = make_uint4(x[0], x[1], x[2], x[3]);
-      *reinterpret_cast<uint4*>(dst + b) = make_uint4(y[0], y[1], y[2], y[3]);
-    }
+  }
+}
+
+template <typename T>
+static void launch_append(const AppendParams& p, bool interleaved, cudaStream_t s) {
+  const int64_t heads = p.n_q_heads + 2 * (int64_t)p.cache.n_kv_heads;
+  const int per = p.cache.head_dim == 64 ? AppendShape<64>::kHeads : AppendShape<128>::kHeads;
+  const int64_t most = 148 * kAppendCtas;
+  const dim3 grid((unsigned)(p.n_tokens < most ? p.n_tokens : most), (unsigned)((heads + per - 1) / per));
+  if (p.cache.head_dim == 64) {
+    if (interleaved) append_kernel<T, 64, true><<<grid, kAppendThreads, 0, s>>>(p);
+    else append_kernel<T, 64, false><<<grid, kAppendThreads, 0, s>>>(p);
+  } else {
+    if (interleaved) append_kernel<T, 128, true><<<grid, kAppendThreads, 0, s>>>(p);
+    else append_kernel<T, 128, false><<<grid, kAppendThreads, 0, s>>>(p);
   }
 }
 
@@ -333,15 +378,9 @@ extern "C" rkv_status rkv_gqa_append(const rkv_gqa_view* cache, int32_t layer, c
   p.q_out = static_cast<uint16_t*>(q_out);
   p.status = d_status;
   cudaStream_t s = (cudaStream_t)stream;
-  const unsigned grid = (unsigned)n_tokens;
   const bool inter = rotary && rotary->interleaved;
-  if (cache->dtype == RKV_GQA_BF16) {
-    if (inter) append_kernel<Bf16, true><<<grid, 128, 0, s>>>(p);
-    else append_kernel<Bf16, false><<<grid, 128, 0, s>>>(p);
-  } else {
-    if (inter) append_kernel<F16, true><<<grid, 128, 0, s>>>(p);
-    else append_kernel<F16, false><<<grid, 128, 0, s>>>(p);
-  }
+  if (cache->dtype == RKV_GQA_BF16) launch_append<Bf16>(p, inter, s);
+  else launch_append<F16>(p, inter, s);
   return check_launch(what);
 }
 

@@ -125,12 +125,6 @@ struct SoftmaxBias {
   static constexpr float kBias = T::kCode == RKV_GQA_F16 ? 7.0f : 0.0f;
 };
 
-// Whether a word of two elements holds an infinity or a NaN.
-template <typename T>
-__device__ __forceinline__ bool not_finite(uint32_t w) {
-  return (w & T::kExpMask) == T::kExpMask || ((w >> 16) & T::kExpMask) == T::kExpMask;
-}
-
 // ---- host helpers (rkv_gqa.cu) ------------------------------------------------------
 // The whole cache as a 2-d tensor map, [rows of 64 of every (layer, page, K or
 // V, head)][head_dim], box 64 lanes x 64 rows (8 KB), 128-byte swizzle.

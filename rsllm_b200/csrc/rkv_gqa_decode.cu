@@ -57,7 +57,8 @@ struct Params {
   int min_units;
   float* part_o;   // [2 * kGrid][rows][head_dim], rows = min(group, 16)
   float* part_ml;  // [2 * kGrid][rows][2]
-  int2* spans;     // [n_seq * n_kv_heads * chunks]: first and last CTA of an item; (-1, -1) written whole
+  int4* joins;     // [kGrid]: the item that begins in a run and does not end there: its first slot (-1: none), last
+                   // run, sequence, and kv head and chunk
   uint16_t* out;
   uint32_t* status;
 };
@@ -195,9 +196,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) decode_kernel(const Para
     if (seen_rows(p, s).pages() == 0) {
       for (int i = tid; i < p.n_q_heads * D / 2; i += kThreads)
         reinterpret_cast<uint32_t*>(p.out)[(int64_t)s * p.n_q_heads * D / 2 + i] = 0u;
-      for (int i = tid; i < hg; i += kThreads) p.spans[(int64_t)s * hg + i] = make_int2(-1, -1);
     }
   }
+  if (tid == 0) p.joins[blockIdx.x] = make_int4(-1, 0, 0, 0);  // unless its last item goes on
   __syncthreads();
   if (u0 >= u1) return;
   int s = (int)found[0];
@@ -436,7 +437,6 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) decode_kernel(const Para
         }
       }
       if (warp == 0) {
-        const int64_t item_id = (int64_t)s * hg + item;
         if (pg == 0 && end == pages) {
           auto norm = [&](int r, float M, float l) {
             const float sink = sink_log2(p.sinks, head0 + r);
@@ -451,7 +451,6 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) decode_kernel(const Para
             if (r0 < live) *reinterpret_cast<uint32_t*>(d0 + 8 * i) = T::pack(o[i][0] * n0, o[i][1] * n0);
             if (r0 + 8 < live) *reinterpret_cast<uint32_t*>(d0 + 8 * D + 8 * i) = T::pack(o[i][2] * n1, o[i][3] * n1);
           }
-          if (lane == 0) p.spans[item_id] = make_int2(-1, -1);
         } else {
           const int64_t slot = 2 * blockIdx.x + (segment > 0);
           float* d0 = p.part_o + (slot * rows + r0) * D + 2 * t4;
@@ -464,11 +463,11 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) decode_kernel(const Para
             if (r0 < live) *reinterpret_cast<float2*>(p.part_ml + 2 * (slot * rows + r0)) = make_float2(M0, L0);
             if (r0 + 8 < live) *reinterpret_cast<float2*>(p.part_ml + 2 * (slot * rows + r0 + 8)) = make_float2(M1, L1);
           }
-          // the run that holds the item's first unit says which runs the join reads
+          // the run that holds the item's first unit says which runs the join reads (thread 0, as above)
           if (lane == 0 && pg == 0) {
             const long long u = u1 - left;  // the item's first unit
             const long long last = ((u + pages) * ctas - 1) / total;
-            p.spans[item_id] = make_int2(2 * blockIdx.x + (segment > 0), (int)last);
+            p.joins[blockIdx.x] = make_int4(2 * blockIdx.x + (segment > 0), (int)last, s, item);
           }
         }
       }
@@ -479,8 +478,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) decode_kernel(const Para
   if (!ok) set_status(p.status, RKV_ERR_CUDA);
 }
 
-// Joins the partial softmaxes of one (item, q head): first slot as recorded,
-// then slot 2 c of every later run c.  A warp takes every sixteenth of them, four
+// Joins the partial softmaxes of one q head of the item that goes on after run c:
+// first slot as recorded, then slot 2 c' of every later run c'.  A warp takes every sixteenth of them, four
 // at a time with their loads out together, lanes the head's lanes; the sixteen
 // sums are added in order.  (One long sequence of 2 kv heads has 148 parts an
 // item: 14 us with eight warps and one load after another.)
@@ -490,11 +489,10 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const Params p) {
   __shared__ float acc[kJoinWarps][D];
   __shared__ float2 ends[kJoinWarps];
   grid_dependency_wait();
-  const int64_t item_id = blockIdx.x;
-  const int hg = p.cache.n_kv_heads * p.chunks;
-  const int64_t s = item_id / hg;
-  const int item = (int)(item_id % hg), r = blockIdx.y;
-  const int2 span = p.spans[item_id];
+  const int4 join = p.joins[blockIdx.x];
+  const int2 span = make_int2(join.x, join.y);
+  const int64_t s = join.z;
+  const int item = join.w, r = blockIdx.y;
   if (span.x < 0 || r >= min(kRows, p.group - (item % p.chunks) * kRows)) return;
   const int rows = min(p.group, kRows);
   const int head = (item / p.chunks) * p.group + (item % p.chunks) * kRows + r;
@@ -572,7 +570,10 @@ static rkv_status launch(const Params& p, const CUtensorMap& map, cudaStream_t s
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(kGrid);
+  // no more CTAs than there can be units
+  const int64_t units = (int64_t)p.n_seq * p.cache.n_kv_heads * p.chunks * p.pt_stride;
+  const unsigned grid = (unsigned)(units < kGrid ? units : kGrid);
+  cfg.gridDim = dim3(grid);
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = Layout<D>::kTotal;
   cfg.stream = s;
@@ -580,7 +581,7 @@ static rkv_status launch(const Params& p, const CUtensorMap& map, cudaStream_t s
   cfg.numAttrs = 1;
   cudaError_t e = cudaLaunchKernelEx(&cfg, decode_kernel<T, D>, p, map);
   if (e == cudaSuccess) {
-    cfg.gridDim = dim3((unsigned)((int64_t)p.n_seq * p.cache.n_kv_heads * p.chunks), (unsigned)(p.group < kRows ? p.group : kRows));
+    cfg.gridDim = dim3(grid, (unsigned)(p.group < kRows ? p.group : kRows));
     cfg.blockDim = dim3(32 * kJoinWarps);
     cfg.dynamicSmemBytes = 0;
     e = cudaLaunchKernelEx(&cfg, join_kernel<T, D>, p);
@@ -600,8 +601,7 @@ extern "C" int64_t rkv_gqa_decode_workspace_bytes(const rkv_gqa_view* cache, int
   using namespace rkv::gqa::dec;
   if (!cache || n_seq < 0 || n_q_heads < 1 || cache->n_kv_heads < 1 || n_q_heads % cache->n_kv_heads != 0) return -1;
   const int64_t group = n_q_heads / cache->n_kv_heads, rows = group < kRows ? group : kRows;
-  const int64_t items = (int64_t)n_seq * cache->n_kv_heads * ((group + kRows - 1) / kRows);
-  return 2 * kGrid * rows * (cache->head_dim + 2) * 4 + items * 8;
+  return 2 * kGrid * rows * (cache->head_dim + 2) * 4 + kGrid * 16;
 }
 
 extern "C" rkv_status rkv_gqa_decode(const rkv_gqa_view* cache, int32_t layer, const void* q, int64_t q_token_stride,
@@ -644,11 +644,9 @@ extern "C" rkv_status rkv_gqa_decode(const rkv_gqa_view* cache, int32_t layer, c
   p.scale_log2 = (float)((double)softmax_scale * 1.4426950408889634);
   p.min_units = 1;
   const int64_t rows = p.group < kRows ? p.group : kRows;
-  if ((int64_t)n_seq * cache->n_kv_heads * p.chunks > INT32_MAX)
-    return fail_shape("n_seq", INT32_MAX, n_seq, "%s: too many sequences", what);
   p.part_o = static_cast<float*>(workspace);
   p.part_ml = p.part_o + 2 * kGrid * rows * cache->head_dim;
-  p.spans = reinterpret_cast<int2*>(p.part_ml + 2 * kGrid * rows * 2);
+  p.joins = reinterpret_cast<int4*>(p.part_ml + 2 * kGrid * rows * 2);
   p.out = static_cast<uint16_t*>(out);
   p.status = d_status;
   CUtensorMap map;

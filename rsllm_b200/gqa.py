@@ -9,7 +9,6 @@ cache; ``GqaKvPool.apply_moves`` does the page copies it decides.
 from __future__ import annotations
 
 import math
-from contextlib import nullcontext
 from ctypes import addressof, c_int32
 
 import numpy as np
@@ -18,6 +17,9 @@ import torch
 from . import _abi
 from ._abi import PAGE_TOKENS
 from .kvcache import CudaError, InvalidArgument, ShapeMismatch, check, raise_status_bits
+
+# The current stream's handle without a Stream object around it, where this torch has it.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 _DTYPES = {torch.bfloat16: _abi.GQA_BF16, torch.float16: _abi.GQA_F16}
 
@@ -95,6 +97,7 @@ class GqaKvPool:
         self.lib = _abi.load()
         self.cache = cache
         self.device = cache.device
+        self._index = cache.get_device()
         self.dtype = cache.dtype
         self.n_layers, self.n_pages, _, self.n_kv_heads, _, self.head_dim = cache.shape
         if status is None:
@@ -107,6 +110,8 @@ class GqaKvPool:
         self._v = addressof(self.view)
         self._s = status.data_ptr()
         self._prefill_ws = self.lib.rkv_gqa_prefill_workspace_bytes(self._v)
+        self._decode_ws = {}  # bytes by number of q heads: they do not grow with the sequences
+        self._scale = 1.0 / math.sqrt(self.head_dim)
 
     # -- status ---------------------------------------------------------------
     def take_status(self, stream: torch.cuda.Stream | None = None) -> int:
@@ -119,10 +124,10 @@ class GqaKvPool:
     def check(self, what: str = "GqaKvPool", stream: torch.cuda.Stream | None = None) -> None:
         raise_status_bits(self.take_status(stream), what)
 
-    # -- argument checks --------------------------------------------------------
+    # -- argument checks (kept short: a small call's time is the host's) ------------
     def _rows(self, t: torch.Tensor, name: str, heads: int | None = None) -> tuple:
-        """(pointer, token stride, head stride) of a [tokens, heads, head_dim] operand."""
-        if not isinstance(t, torch.Tensor) or t.dtype != self.dtype or t.device != self.device:
+        """(pointer, token stride, head stride, shape) of a [tokens, heads, head_dim] operand."""
+        if not isinstance(t, torch.Tensor) or t.dtype is not self.dtype or t.get_device() != self._index:
             raise ShapeMismatch(f"{name}: expected a {self.dtype} tensor on {self.device}")
         shape, stride = t.shape, t.stride()
         if len(shape) != 3 or shape[2] != self.head_dim or (heads is not None and shape[1] != heads):
@@ -131,45 +136,47 @@ class GqaKvPool:
             raise ShapeMismatch(f"{name}: the {self.head_dim} elements of a row must be contiguous")
         # a stride that no second row uses may be anything
         return (t.data_ptr(), stride[0] if shape[0] > 1 else shape[1] * shape[2],
-                stride[1] if shape[1] > 1 else shape[2])
+                stride[1] if shape[1] > 1 else shape[2], shape)
 
     def _need(self, t: torch.Tensor, dtype: torch.dtype, name: str, shape: tuple) -> int:
-        if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.device != self.device:
+        if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.get_device() != self._index:
             raise ShapeMismatch(f"{name}: expected a {dtype} tensor on {self.device}")
-        if tuple(t.shape) != shape or not t.is_contiguous():
-            raise ShapeMismatch(f"{name}: expected a contiguous {shape} tensor, got {tuple(t.shape)}")
+        if t.shape != shape or not t.is_contiguous():
+            raise ShapeMismatch(f"{name}: expected a contiguous {tuple(shape)} tensor, got {tuple(t.shape)}")
         return t.data_ptr()
 
     def _table(self, page_table: torch.Tensor, n_seq: int) -> tuple:
         if page_table.dim() != 2:
             raise ShapeMismatch("page_table: expected [n_seq, stride]")
-        return self._need(page_table, torch.int32, "page_table", (n_seq, page_table.shape[1])), page_table.shape[1]
+        stride = page_table.shape[1]
+        return self._need(page_table, torch.int32, "page_table", (n_seq, stride)), stride
 
-    def _out(self, out: torch.Tensor | None, like: torch.Tensor, name: str, stream) -> tuple:
+    def _empty(self, shape, dtype: torch.dtype, stream) -> torch.Tensor:
+        """Memory made for a call belongs to the stream that the call runs on."""
+        if stream is None:
+            return torch.empty(shape, dtype=dtype, device=self.device)
+        with torch.cuda.stream(stream):
+            return torch.empty(shape, dtype=dtype, device=self.device)
+
+    def _out(self, out: torch.Tensor | None, shape, name: str, stream) -> tuple:
         if out is None:
-            with self._on(stream):
-                out = torch.empty(like.shape, dtype=self.dtype, device=self.device)
+            out = self._empty(shape, self.dtype, stream)
             return out, out.data_ptr()
-        return out, self._need(out, self.dtype, name, tuple(like.shape))
+        return out, self._need(out, self.dtype, name, shape)
 
     def _workspace(self, workspace: torch.Tensor | None, nbytes: int, stream) -> tuple:
-        if nbytes <= 0:
-            return None, 0
         if workspace is None:
-            with self._on(stream):
-                workspace = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
-        elif workspace.device != self.device or not workspace.is_contiguous() or \
+            workspace = self._empty(nbytes, torch.uint8, stream)
+        elif workspace.get_device() != self._index or not workspace.is_contiguous() or \
                 workspace.numel() * workspace.element_size() < nbytes:
             raise ShapeMismatch(f"workspace: expected a contiguous tensor of {nbytes} bytes on {self.device}")
         return workspace, workspace.data_ptr()
 
-    @staticmethod
-    def _on(stream):
-        """Memory made for a call belongs to the stream that the call runs on."""
-        return nullcontext() if stream is None else torch.cuda.stream(stream)
-
     def _stream(self, stream) -> int:
-        return stream.cuda_stream if stream is not None else torch.cuda.current_stream(self.device).cuda_stream
+        if stream is not None:
+            return stream.cuda_stream
+        return _raw_stream(self._index) if _raw_stream is not None else \
+            torch.cuda.current_stream(self.device).cuda_stream
 
     # -- append -------------------------------------------------------------------
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, slot_mapping: torch.Tensor,
@@ -181,15 +188,15 @@ class GqaKvPool:
         k is rotated by the positions ``pos`` (int32 ``[tokens]``, or
         ``[axes, tokens]``), and q ``[tokens, n_q_heads, head_dim]``, if given,
         too: the rotated q is returned (``rkv_gqa_append``)."""
-        kp, k_ts, k_hs = self._rows(k, "k", self.n_kv_heads)
-        vp, v_ts, v_hs = self._rows(v, "v", self.n_kv_heads)
-        n = k.shape[0]
-        if v.shape[0] != n:
+        kp, k_ts, k_hs, shape = self._rows(k, "k", self.n_kv_heads)
+        vp, v_ts, v_hs, v_shape = self._rows(v, "v", self.n_kv_heads)
+        n = shape[0]
+        if v_shape[0] != n:
             raise ShapeMismatch("append: k and v differ in tokens")
         slots = self._need(slot_mapping, torch.int32, "slot_mapping", (n,))
         qp = q_ts = q_hs = heads = op = posp = 0
         if rotary is not None:
-            if rotary.table.device != self.device:
+            if rotary.table.get_device() != self._index:
                 raise ShapeMismatch("append: the rotary table is on another device")
             axes = len(rotary.sections)
             if pos is None:
@@ -198,11 +205,11 @@ class GqaKvPool:
         if q is not None:
             if rotary is None:
                 raise InvalidArgument("append: q is only taken with rotary")
-            qp, q_ts, q_hs = self._rows(q, "q")
-            if q.shape[0] != n:
+            qp, q_ts, q_hs, q_shape = self._rows(q, "q")
+            if q_shape[0] != n:
                 raise ShapeMismatch("append: q and k differ in tokens")
-            heads = q.shape[1]
-            q_out, op = self._out(q_out, q, "q_out", stream)
+            heads = q_shape[1]
+            q_out, op = self._out(q_out, q_shape, "q_out", stream)
         check(self.lib.rkv_gqa_append(self._v, layer, kp, k_ts, k_hs, vp, v_ts, v_hs, n, slots,
                                       rotary._p if rotary is not None else 0, posp, qp, q_ts, q_hs, heads, op, self._s,
                                       self._stream(stream)), "append")
@@ -217,16 +224,16 @@ class GqaKvPool:
         head_dim]`` (sequence s: rows ``cu_q[s]`` to ``cu_q[s + 1]``) over the
         ``kv_lens[s]`` rows of each sequence, which end with the new tokens'
         own (``rkv_gqa_prefill``).  The scale defaults to 1/sqrt(head_dim)."""
-        qp, q_ts, q_hs = self._rows(q, "q")
-        n, heads = q.shape[0], q.shape[1]
+        qp, q_ts, q_hs, shape = self._rows(q, "q")
+        n, heads = shape[0], shape[1]
         n_seq = kv_lens.shape[0] if kv_lens.dim() == 1 else -1
         lens = self._need(kv_lens, torch.int32, "kv_lens", (n_seq,))
         cu = self._need(cu_q, torch.int32, "cu_q", (n_seq + 1,))
         table, stride = self._table(page_table, n_seq)
         sink = 0 if sinks is None else self._need(sinks, torch.float32, "sinks", (heads,))
         ws, wp = self._workspace(workspace, self._prefill_ws, stream)
-        out, op = self._out(out, q, "out", stream)
-        scale = 1.0 / math.sqrt(self.head_dim) if softmax_scale is None else softmax_scale
+        out, op = self._out(out, shape, "out", stream)
+        scale = self._scale if softmax_scale is None else softmax_scale
         check(self.lib.rkv_gqa_prefill(self._v, layer, qp, q_ts, q_hs, n, heads, cu, n_seq, table, stride, lens, window,
                                        sink, scale, wp, op, self._s, self._stream(stream)), "prefill")
         return out
@@ -238,14 +245,16 @@ class GqaKvPool:
         """Attention of one new token per sequence, q ``[n_seq, n_q_heads,
         head_dim]``, over its ``kv_lens[s]`` rows, the token's own (appended
         before) being the last (``rkv_gqa_decode``)."""
-        qp, q_ts, q_hs = self._rows(q, "q")
-        n_seq, heads = q.shape[0], q.shape[1]
+        qp, q_ts, q_hs, shape = self._rows(q, "q")
+        n_seq, heads = shape[0], shape[1]
         lens = self._need(kv_lens, torch.int32, "kv_lens", (n_seq,))
         table, stride = self._table(page_table, n_seq)
         sink = 0 if sinks is None else self._need(sinks, torch.float32, "sinks", (heads,))
-        ws, wp = self._workspace(workspace, self.lib.rkv_gqa_decode_workspace_bytes(self._v, n_seq, heads), stream)
-        out, op = self._out(out, q, "out", stream)
-        scale = 1.0 / math.sqrt(self.head_dim) if softmax_scale is None else softmax_scale
+        if heads not in self._decode_ws:
+            self._decode_ws[heads] = max(0, self.lib.rkv_gqa_decode_workspace_bytes(self._v, n_seq, heads))
+        ws, wp = self._workspace(workspace, self._decode_ws[heads], stream)
+        out, op = self._out(out, shape, "out", stream)
+        scale = self._scale if softmax_scale is None else softmax_scale
         check(self.lib.rkv_gqa_decode(self._v, layer, qp, q_ts, q_hs, n_seq, heads, table, stride, lens, window, sink,
                                       scale, wp, op, self._s, self._stream(stream)), "decode")
         return out
@@ -277,7 +286,7 @@ class GqaKvPool:
     def _move(self, src: np.ndarray, dst: np.ndarray, stream) -> None:
         if not src.size:
             return
-        with self._on(stream):
+        with torch.cuda.stream(stream):  # None: the current one
             both = torch.from_numpy(np.stack((src, dst))).to(self.device)
             self.copy_pages(both[0], both[1], stream)
 
