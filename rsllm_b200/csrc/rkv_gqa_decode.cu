@@ -12,8 +12,9 @@
 //   * A unit of work is one page (64 rows) of one kv head: its K and its V are
 //     8 or 16 KB of contiguous memory each.  The units of all sequences in
 //     (sequence, kv head, page) order are cut into equal runs, one per CTA, so
-//     ragged lengths, which only the device knows, leave no CTA idle.  A run
-//     may begin and end inside a (sequence, kv head); such ends are written as
+//     ragged lengths, which only the device knows, leave no CTA idle.  Beginning
+//     and ending a (sequence, kv head) costs some 3 us, and counts as so many
+//     pages.  A run may begin and end inside one; such ends are written as
 //     partial softmaxes (m, l, O) and joined by a second small kernel, in the
 //     order of the rows.
 //   * A producer warp keeps a ring of pages in shared memory full (tensor-map
@@ -54,7 +55,6 @@ struct Params {
   int window;
   const float* sinks;
   float scale_log2;
-  int min_units;
   float* part_o;   // [2 * kGrid][rows][head_dim], rows = min(group, 16)
   float* part_ml;  // [2 * kGrid][rows][2]
   int4* joins;     // [kGrid]: the item that begins in a run and does not end there: its first slot (-1: none), last
@@ -68,6 +68,16 @@ struct Seen {
   int lo, hi;
   __device__ int first_page() const { return lo / kPage; }
   __device__ int pages() const { return hi > lo ? (hi + kPage - 1) / kPage - lo / kPage : 0; }
+  // an item's units: its pages behind what beginning and ending it costs (256 ragged sequences: runs of 13 items ended
+  // at 134 us and runs of 3 at 104 when only pages counted)
+  template <int D>
+  __device__ int units() const {
+    return hi > lo ? pages() + item_units<D>() : 0;
+  }
+  template <int D>
+  static __device__ constexpr int item_units() {
+    return D == 64 ? 4 : 2;
+  }
 };
 __device__ __forceinline__ Seen seen_rows(const Params& p, int s) {
   const int most = (int)p.pt_stride * kPage;
@@ -157,7 +167,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) decode_kernel(const Para
   const int per = (p.n_seq + kThreads - 1) / kThreads;
   const int s_begin = min(tid * per, p.n_seq), s_end = min(s_begin + per, p.n_seq);
   long long mine = 0;
-  for (int s = s_begin; s < s_end; ++s) mine += seen_rows(p, s).pages();
+  for (int s = s_begin; s < s_end; ++s) mine += seen_rows(p, s).template units<D>();
   long long upto = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -173,7 +183,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) decode_kernel(const Para
   }
   const int hg = p.cache.n_kv_heads * p.chunks;  // items of a sequence
   total *= hg;
-  const long long ctas = max(1ll, min((long long)gridDim.x, total / p.min_units));
+  const long long ctas = max(1ll, min((long long)gridDim.x, total));
   const long long u0 = blockIdx.x < ctas ? blockIdx.x * total / ctas : total;
   const long long u1 = blockIdx.x < ctas ? (blockIdx.x + 1) * total / ctas : total;
   long long* found = scan + 5;
@@ -182,7 +192,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) decode_kernel(const Para
     long long at = before;
     int s = s_begin;
     for (; s < s_end; ++s) {
-      const int n = seen_rows(p, s).pages();
+      const int n = seen_rows(p, s).template units<D>();
       if (u0 < (at + n) * hg) break;
       at += n;
     }
@@ -215,11 +225,13 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) decode_kernel(const Para
       const Seen see = seen_rows(p, s);
       const int pages = see.pages();
       if (pages == 0) continue;
-      for (int item = (int)(rest / pages), pg = (int)(rest % pages); item < hg && left > 0 && ok; ++item, pg = 0) {
+      const int units = see.units<D>();
+      for (int item = (int)(rest / units), x = (int)(rest % units); item < hg && left > 0 && ok; ++item, x = 0) {
         const int head = item / p.chunks;
         const int32_t* ids = p.page_table + s * p.pt_stride + see.first_page();
-        const int end = (int)min((long long)pages, pg + left);
-        left -= end - pg;
+        const int stop = (int)min((long long)units, x + left);
+        const int pg = max(0, x - see.item_units<D>()), end = max(0, stop - see.item_units<D>());
+        left -= stop - x;
         for (int at = pg; at < end && ok; at += 32) {
           const int id = at + lane < end ? __ldg(ids + at + lane) : 0;
           const bool good = id >= 0 && id < p.cache.n_pages;
@@ -271,8 +283,13 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) decode_kernel(const Para
     const Seen see = seen_rows(p, s);
     const int pages = see.pages();
     if (pages == 0) continue;
-    for (int item = (int)(rest / pages), pg = (int)(rest % pages); item < hg && left > 0 && ok; ++item, pg = 0, ++segment) {
-      const int end = (int)min((long long)pages, pg + left);
+    const int units = see.units<D>();
+    for (int item = (int)(rest / units), x = (int)(rest % units); item < hg && left > 0 && ok; ++item, x = 0) {
+      const int stop = (int)min((long long)units, x + left);
+      const int pg = max(0, x - see.item_units<D>()), end = max(0, stop - see.item_units<D>());
+      const long long begin = u1 - left - x;  // the item's first unit
+      left -= stop - x;
+      if (end <= pg) continue;
       const int head0 = (item / p.chunks) * p.group + (item % p.chunks) * kRows;  // first q head
       const int live = min(kRows, p.group - (item % p.chunks) * kRows);
       uint32_t qf[kK][4];
@@ -465,49 +482,50 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) decode_kernel(const Para
           }
           // the run that holds the item's first unit says which runs the join reads (thread 0, as above)
           if (lane == 0 && pg == 0) {
-            const long long u = u1 - left;  // the item's first unit
-            const long long last = ((u + pages) * ctas - 1) / total;
+            const long long last = ((begin + units) * ctas - 1) / total;  // its last unit is a page
             p.joins[blockIdx.x] = make_int4(2 * blockIdx.x + (segment > 0), (int)last, s, item);
           }
         }
       }
-      left -= end - pg;
+      ++segment;
     }
     rest = 0;
   }
   if (!ok) set_status(p.status, RKV_ERR_CUDA);
 }
 
-// Joins the partial softmaxes of one q head of the item that goes on after run c:
-// first slot as recorded, then slot 2 c' of every later run c'.  A warp takes every sixteenth of them, four
-// at a time with their loads out together, lanes the head's lanes; the sixteen
-// sums are added in order.  (One long sequence of 2 kv heads has 148 parts an
-// item: 14 us with eight warps and one load after another.)
-constexpr int kJoinWarps = 16;
-template <typename T, int D>
-__global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const Params p) {
-  __shared__ float acc[kJoinWarps][D];
-  __shared__ float2 ends[kJoinWarps];
+// Joins the partial softmaxes of the q heads of the item that goes on after run
+// c: first slot as recorded, then slot 2 c' of every later run c'.  kWarps warps
+// take the parts of a head in turn, four at a time with their loads out together,
+// lanes the head's lanes; the warps' sums are added in order.  Sixteen warps where
+// an item has many parts (one sequence of 131072 rows and 2 kv heads: 148; 14 us
+// with eight warps and one load after another, 6 with sixteen), one where it has
+// a few (256 ragged sequences: 13.5 us with sixteen, whose threads mostly start
+// for nothing).
+constexpr int kJoinThreads = 128;  // with one warp a head: four heads
+template <typename T, int D, int kWarps>
+__global__ void __launch_bounds__(kWarps == 1 ? kJoinThreads : 32 * kWarps) join_kernel(const Params p) {
+  __shared__ float acc[kWarps == 1 ? 1 : kWarps][D];
+  __shared__ float2 ends[kWarps];
   grid_dependency_wait();
   const int4 join = p.joins[blockIdx.x];
-  const int2 span = make_int2(join.x, join.y);
+  const int warp = kWarps == 1 ? 0 : threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t s = join.z;
-  const int item = join.w, r = blockIdx.y;
-  if (span.x < 0 || r >= min(kRows, p.group - (item % p.chunks) * kRows)) return;
+  const int item = join.w, r = kWarps == 1 ? blockIdx.y * (kJoinThreads / 32) + (threadIdx.x >> 5) : blockIdx.y;
+  if (join.x < 0 || r >= min(kRows, p.group - (item % p.chunks) * kRows)) return;
   const int rows = min(p.group, kRows);
   const int head = (item / p.chunks) * p.group + (item % p.chunks) * kRows + r;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int count = span.y - span.x / 2 + 1;
-  auto slot = [&](int i) { return (int64_t)(i == 0 ? span.x : 2 * (span.x / 2 + i)); };
+  const int count = join.y - join.x / 2 + 1;
+  auto slot = [&](int i) { return (int64_t)(i == 0 ? join.x : 2 * (join.x / 2 + i)); };
   constexpr int kAhead = 4;
   float o[D / 32] = {};
   float m = -INFINITY, l = 0.f;
-  for (int i0 = warp; i0 < count; i0 += kAhead * kJoinWarps) {
+  for (int i0 = warp; i0 < count; i0 += kAhead * kWarps) {
     float2 e[kAhead];
     float v[kAhead][D / 32];
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
-      const int i = i0 + k * kJoinWarps;
+      const int i = i0 + k * kWarps;
       e[k] = make_float2(-INFINITY, 0.f);
       if (i >= count) continue;
       const int64_t at = slot(i) * rows + r;
@@ -531,26 +549,35 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const Params p) {
       m = top;
     }
   }
-#pragma unroll
-  for (int j = 0; j < D / 32; ++j) acc[warp][D / 32 * lane + j] = o[j];
-  if (lane == 0) ends[warp] = make_float2(m, l);
-  __syncthreads();
-  if (threadIdx.x < D / 2) {
-    const float sink = sink_log2(p.sinks, head);
-    float top = sink;
-#pragma unroll
-    for (int w = 0; w < kJoinWarps; ++w) top = fmaxf(top, ends[w].x);
+  const float sink = sink_log2(p.sinks, head);
+  uint32_t* const out = reinterpret_cast<uint32_t*>(p.out + (s * p.n_q_heads + head) * D);
+  if constexpr (kWarps == 1) {
+    float top = fmaxf(m, sink);
     if (top == -INFINITY) top = 0.f;
-    float a = 0.f, b = 0.f, total = ex2(sink - top);
+    const float f = ex2(m - top), total = l * f + ex2(sink - top), inv = total == 0.f ? 0.f : f / total;
 #pragma unroll
-    for (int w = 0; w < kJoinWarps; ++w) {
-      const float f = ex2(ends[w].x - top);
-      a += f * acc[w][2 * threadIdx.x];
-      b += f * acc[w][2 * threadIdx.x + 1];
-      total += f * ends[w].y;
+    for (int j = 0; j < D / 64; ++j) out[D / 64 * lane + j] = T::pack(o[2 * j] * inv, o[2 * j + 1] * inv);
+  } else {
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j) acc[warp][D / 32 * lane + j] = o[j];
+    if (lane == 0) ends[warp] = make_float2(m, l);
+    __syncthreads();
+    if (threadIdx.x < D / 2) {
+      float top = sink;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) top = fmaxf(top, ends[w].x);
+      if (top == -INFINITY) top = 0.f;
+      float a = 0.f, b = 0.f, total = ex2(sink - top);
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float f = ex2(ends[w].x - top);
+        a += f * acc[w][2 * threadIdx.x];
+        b += f * acc[w][2 * threadIdx.x + 1];
+        total += f * ends[w].y;
+      }
+      const float inv = total == 0.f ? 0.f : 1.f / total;
+      out[threadIdx.x] = T::pack(a * inv, b * inv);
     }
-    const float inv = total == 0.f ? 0.f : 1.f / total;
-    reinterpret_cast<uint32_t*>(p.out + (s * p.n_q_heads + head) * D)[threadIdx.x] = T::pack(a * inv, b * inv);
   }
 }
 
@@ -581,10 +608,18 @@ static rkv_status launch(const Params& p, const CUtensorMap& map, cudaStream_t s
   cfg.numAttrs = 1;
   cudaError_t e = cudaLaunchKernelEx(&cfg, decode_kernel<T, D>, p, map);
   if (e == cudaSuccess) {
-    cfg.gridDim = dim3(grid, (unsigned)(p.group < kRows ? p.group : kRows));
-    cfg.blockDim = dim3(32 * kJoinWarps);
+    const unsigned rows = (unsigned)(p.group < kRows ? p.group : kRows);
+    const int64_t items = (int64_t)p.n_seq * p.cache.n_kv_heads * p.chunks;
     cfg.dynamicSmemBytes = 0;
-    e = cudaLaunchKernelEx(&cfg, join_kernel<T, D>, p);
+    if (grid > 8 * items) {  // more than eight parts an item, were they alike
+      cfg.gridDim = dim3(grid, rows);
+      cfg.blockDim = dim3(32 * 16);
+      e = cudaLaunchKernelEx(&cfg, join_kernel<T, D, 16>, p);
+    } else {
+      cfg.gridDim = dim3(grid, (rows + kJoinThreads / 32 - 1) / (kJoinThreads / 32));
+      cfg.blockDim = dim3(kJoinThreads);
+      e = cudaLaunchKernelEx(&cfg, join_kernel<T, D, 1>, p);
+    }
   }
   if (e != cudaSuccess) {
     cudaGetLastError();
@@ -642,7 +677,6 @@ extern "C" rkv_status rkv_gqa_decode(const rkv_gqa_view* cache, int32_t layer, c
   p.window = window;
   p.sinks = sinks;
   p.scale_log2 = (float)((double)softmax_scale * 1.4426950408889634);
-  p.min_units = 1;
   const int64_t rows = p.group < kRows ? p.group : kRows;
   p.part_o = static_cast<float*>(workspace);
   p.part_ml = p.part_o + 2 * kGrid * rows * cache->head_dim;
