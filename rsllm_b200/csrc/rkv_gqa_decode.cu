@@ -57,8 +57,8 @@ struct Params {
   float scale_log2;
   float* part_o;   // [2 * kGrid][rows][head_dim], rows = min(group, 16)
   float* part_ml;  // [2 * kGrid][rows][2]
-  int4* joins;     // [kGrid]: the item that begins in a run and does not end there: its first slot (-1: none), last
-                   // run, sequence, and kv head and chunk
+  int by_item;     // joins has an entry for each item (fewer than the runs), else for each run, whose last item it is
+  int4* joins;     // [kGrid]: first slot of a shared item (-1: none), last run, sequence, and kv head and chunk
   uint16_t* out;
   uint32_t* status;
 };
@@ -206,9 +206,11 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) decode_kernel(const Para
     if (seen_rows(p, s).pages() == 0) {
       for (int i = tid; i < p.n_q_heads * D / 2; i += kThreads)
         reinterpret_cast<uint32_t*>(p.out)[(int64_t)s * p.n_q_heads * D / 2 + i] = 0u;
+      if (p.by_item)
+        for (int i = tid; i < hg; i += kThreads) p.joins[s * hg + i] = make_int4(-1, 0, 0, 0);
     }
   }
-  if (tid == 0) p.joins[blockIdx.x] = make_int4(-1, 0, 0, 0);  // unless its last item goes on
+  if (tid == 0 && !p.by_item) p.joins[blockIdx.x] = make_int4(-1, 0, 0, 0);  // unless its last item goes on
   __syncthreads();
   if (u0 >= u1) return;
   int s = (int)found[0];
@@ -468,6 +470,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) decode_kernel(const Para
             if (r0 < live) *reinterpret_cast<uint32_t*>(d0 + 8 * i) = T::pack(o[i][0] * n0, o[i][1] * n0);
             if (r0 + 8 < live) *reinterpret_cast<uint32_t*>(d0 + 8 * D + 8 * i) = T::pack(o[i][2] * n1, o[i][3] * n1);
           }
+          if (lane == 0 && p.by_item) p.joins[s * hg + item] = make_int4(-1, 0, 0, 0);
         } else {
           const int64_t slot = 2 * blockIdx.x + (segment > 0);
           float* d0 = p.part_o + (slot * rows + r0) * D + 2 * t4;
@@ -483,7 +486,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) decode_kernel(const Para
           // the run that holds the item's first unit says which runs the join reads (thread 0, as above)
           if (lane == 0 && pg == 0) {
             const long long last = ((begin + units) * ctas - 1) / total;  // its last unit is a page
-            p.joins[blockIdx.x] = make_int4(2 * blockIdx.x + (segment > 0), (int)last, s, item);
+            p.joins[p.by_item ? s * hg + item : blockIdx.x] = make_int4(2 * blockIdx.x + (segment > 0), (int)last, s, item);
           }
         }
       }
@@ -494,8 +497,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) decode_kernel(const Para
   if (!ok) set_status(p.status, RKV_ERR_CUDA);
 }
 
-// Joins the partial softmaxes of the q heads of the item that goes on after run
-// c: first slot as recorded, then slot 2 c' of every later run c'.  kWarps warps
+// Joins the partial softmaxes of the q heads of a shared item: first slot as
+// recorded, then slot 2 c' of every later run c'.  kWarps warps
 // take the parts of a head in turn, four at a time with their loads out together,
 // lanes the head's lanes; the warps' sums are added in order.  Sixteen warps where
 // an item has many parts (one sequence of 131072 rows and 2 kv heads: 148; 14 us
@@ -582,7 +585,7 @@ __global__ void __launch_bounds__(kWarps == 1 ? kJoinThreads : 32 * kWarps) join
 }
 
 template <typename T, int D>
-static rkv_status launch(const Params& p, const CUtensorMap& map, cudaStream_t s, const char* what) {
+static rkv_status launch(Params p, const CUtensorMap& map, cudaStream_t s, const char* what) {
   static std::atomic<bool> ready[kMaxDevicesCached];  // the shared-memory opt-in is per device
   int dev = 0;
   cudaGetDevice(&dev);
@@ -600,6 +603,8 @@ static rkv_status launch(const Params& p, const CUtensorMap& map, cudaStream_t s
   // no more CTAs than there can be units
   const int64_t units = (int64_t)p.n_seq * p.cache.n_kv_heads * p.chunks * p.pt_stride;
   const unsigned grid = (unsigned)(units < kGrid ? units : kGrid);
+  const int64_t items = (int64_t)p.n_seq * p.cache.n_kv_heads * p.chunks;
+  p.by_item = grid > 8 * items;  // more than eight parts an item, were they alike
   cfg.gridDim = dim3(grid);
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = Layout<D>::kTotal;
@@ -609,10 +614,9 @@ static rkv_status launch(const Params& p, const CUtensorMap& map, cudaStream_t s
   cudaError_t e = cudaLaunchKernelEx(&cfg, decode_kernel<T, D>, p, map);
   if (e == cudaSuccess) {
     const unsigned rows = (unsigned)(p.group < kRows ? p.group : kRows);
-    const int64_t items = (int64_t)p.n_seq * p.cache.n_kv_heads * p.chunks;
     cfg.dynamicSmemBytes = 0;
-    if (grid > 8 * items) {  // more than eight parts an item, were they alike
-      cfg.gridDim = dim3(grid, rows);
+    if (p.by_item) {
+      cfg.gridDim = dim3((unsigned)items, rows);
       cfg.blockDim = dim3(32 * 16);
       e = cudaLaunchKernelEx(&cfg, join_kernel<T, D, 16>, p);
     } else {
