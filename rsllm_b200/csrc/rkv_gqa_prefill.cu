@@ -418,74 +418,83 @@ prefill_kernel(const Params p, const __grid_constant__ CUtensorMap map, const __
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
     if (warp == kPlanWarp) {
       // ---------------------------------------------------------------- planner
-      if (lane == 0) {
-        Job* out = reinterpret_cast<Job*>(smem + L::kJob);
-        bool ok = true;
-        int n = 0;
-        auto hand_out = [&](const Job& w) {
-          const int at = n % kJobs;
-          // as long as the work before takes: twenty of the usual limits
-          for (int i = 0; n >= kJobs && !(ok = mbar_wait(bars + L::kBarJob + 8 * (kJobs + at), (n / kJobs - 1) & 1, abort_flag)); ++i)
-            if (i == 20 || *abort_flag) return;
+      // The whole warp computes the same, but for the search; lane 0 writes.
+      Job* out = reinterpret_cast<Job*>(smem + L::kJob);
+      bool ok = true;
+      int n = 0;
+      auto hand_out = [&](const Job& w) {
+        const int at = n % kJobs;
+        // as long as the work before takes: twenty of the usual limits
+        for (int i = 0; n >= kJobs && !(ok = __all_sync(0xffffffffu, mbar_wait(bars + L::kBarJob + 8 * (kJobs + at), (n / kJobs - 1) & 1, abort_flag))); ++i)
+          if (i == 20 || __any_sync(0xffffffffu, *abort_flag)) return;
+        if (lane == 0) {
           out[at] = w;
           mbar_arrive(bars + L::kBarJob + 8 * at);
-          ++n;
-        };
-        int4 first = make_int4(0, 0, 0, 0), last = first;  // what the two slots hold
-        long long left = u1 - u0;
-        if (left > 0) {
-          int s = *start_seq;
-          long long off = *start_off;
-          for (; left > 0 && ok; ++s, off = 0) {
-            Blocks b;
-            b.init(p, s);
-            const long long per_head = b.before(b.count);
-            if (per_head == 0) continue;
-            int head = (int)(off / per_head);
+        }
+        ++n;
+      };
+      int4 first = make_int4(0, 0, 0, 0), last = first;  // what the two slots hold
+      long long left = u1 - u0;
+      if (left > 0) {
+        int s = *start_seq;
+        long long off = *start_off;
+        for (; left > 0 && ok; ++s, off = 0) {
+          Blocks b;
+          b.init(p, s);
+          const long long per_head = b.before(b.count);
+          if (per_head == 0) continue;
+          int head = 0;
+          if (off >= per_head) {
+            head = (int)(off / per_head);
             off -= head * per_head;
-            int lo = 0, hi = b.count;  // the block that holds `off`
-            while (hi - lo > 1) {
-              const int mid = (lo + hi) / 2;
-              if (b.before(mid) <= off) lo = mid;
-              else hi = mid;
-            }
-            long long x = off - b.before(lo);
-            for (; head < p.cache.n_kv_heads && left > 0 && ok; ++head, lo = 0) {
-              for (int i = lo; i < b.count && left > 0 && ok; ++i, x = 0) {
-                const long long cost = b.cost(i), stop = min(cost, x + left);
-                const int steps = b.steps(i), k0 = cut_step(x, cost, steps), k1 = cut_step(stop, cost, steps);
-                if (k1 > k0 || (steps == 0 && x == 0)) {
-                  Job w;
-                  w.head = head;
-                  w.seq = s;
-                  w.token = b.token + i * b.span;
-                  w.tokens = min(b.span, b.tokens - i * b.span);
-                  w.pos = b.pos + i * b.span;
-                  w.len = b.len;
-                  w.step0 = b.first_step(i) + k0;
-                  w.steps = k1 - k0;
-                  const int end0 = w.pos + min(w.tokens, p.tile_tokens);
-                  w.steps0 = max(0, min(w.steps, (end0 > 0 ? (end0 + kN - 1) / kN : 0) - w.step0));
-                  w.slot = -1;
-                  if (k1 - k0 < steps) {
-                    w.slot = 2 * blockIdx.x + (k0 == 0);
-                    (k0 == 0 ? last : first) = make_int4(w.token, w.tokens, head, k1 == steps ? 3 : 1);
-                  }
-                  hand_out(w);
+          }
+          int lo = 0, hi = b.count;  // the block that holds `off` is in [lo, hi): 32 places are looked at together
+          while (off > 0 && hi - lo > 1) {
+            const int step = (hi - lo + 31) / 32;
+            const int at = min(lo + lane * step, hi - 1);
+            const unsigned below = __ballot_sync(0xffffffffu, b.before(at) <= off);  // lanes from 0 on
+            const int k = 31 - __clz(below);
+            const int from = min(lo + k * step, hi - 1);
+            hi = min(hi, from + step);
+            lo = from;
+          }
+          long long x = off - b.before(lo);
+          for (; head < p.cache.n_kv_heads && left > 0 && ok; ++head, lo = 0) {
+            for (int i = lo; i < b.count && left > 0 && ok; ++i, x = 0) {
+              const long long cost = b.cost(i), stop = min(cost, x + left);
+              const int steps = b.steps(i), k0 = cut_step(x, cost, steps), k1 = cut_step(stop, cost, steps);
+              if (k1 > k0 || (steps == 0 && x == 0)) {
+                Job w;
+                w.head = head;
+                w.seq = s;
+                w.token = b.token + i * b.span;
+                w.tokens = min(b.span, b.tokens - i * b.span);
+                w.pos = b.pos + i * b.span;
+                w.len = b.len;
+                w.step0 = b.first_step(i) + k0;
+                w.steps = k1 - k0;
+                const int end0 = w.pos + min(w.tokens, p.tile_tokens);
+                w.steps0 = max(0, min(w.steps, (end0 > 0 ? (end0 + kN - 1) / kN : 0) - w.step0));
+                w.slot = -1;
+                if (k1 - k0 < steps) {
+                  w.slot = 2 * blockIdx.x + (k0 == 0);
+                  (k0 == 0 ? last : first) = make_int4(w.token, w.tokens, head, k1 == steps ? 3 : 1);
                 }
-                left -= stop - x;
+                hand_out(w);
               }
+              left -= stop - x;
             }
           }
         }
+      }
+      if (lane == 0) {
         p.parts[2 * blockIdx.x] = first;
         p.parts[2 * blockIdx.x + 1] = last;
-        Job w = {};
-        w.steps = -1;
-        if (ok) hand_out(w);
-        if (!ok) give_up();
       }
-      __syncwarp();
+      Job w = {};
+      w.steps = -1;
+      if (ok) hand_out(w);
+      if (!ok) give_up();
     } else if (warp < kMmaWarp + 2) {
       // ----------------------------------------------------------- MMA issuers
       // The whole warp waits, so that it stays converged; one lane issues.
