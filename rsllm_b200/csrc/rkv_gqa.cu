@@ -130,7 +130,9 @@ struct AppendParams {
 // Bytes bound it -- every row once in and once out -- if the instructions are few
 // and the bytes on their way many: a token's slot and positions are loaded while
 // the one before is worked on, so that its rows and its cosines and sines are
-// one trip to memory together.
+// one trip to memory together.  20011 tokens of 28 + 4 + 4 heads of 128, three
+// axes, f16: 82 us, 4.57 TB/s (101 to 133 us where every thread worked out its heads
+// and the axes of its pairs for every token: 67 instead of 41 million instructions).
 constexpr int kAppendThreads = 128, kAhead = 3, kAppendCtas = 6;
 template <int D>
 struct AppendShape {
@@ -278,6 +280,7 @@ constexpr int kCopyThreads = 256;
 constexpr int kCopyChunk = kCopyThreads * 4 * 16;  // 16 KB: four 16-byte vectors a thread, loads before stores
 
 // One CTA per (pair, layer, 16 KB of the page); pages are multiples of 16 KB.
+// Bytes bound it: 2500 pages of 256 KB take 203 us, 6.45 TB/s, the rate of a copy.
 __global__ void __launch_bounds__(kCopyThreads)
 copy_kernel(rkv_gqa_view c, int64_t page_bytes, int chunks, const int32_t* __restrict__ src,
             const int32_t* __restrict__ dst, uint32_t* __restrict__ status) {

@@ -49,11 +49,12 @@
 // Measured and not kept: two sets of softmax warps taking a tile's steps in
 // turn (head_dim 128: 539 us instead of 527 for 8192 tokens; head_dim 64: 5%
 // faster); the tiles' warps handing each other the exponentials by named barriers
-// (550); a cubic on the FMA pipe for a quarter of the exponentials (+2%, for half
-// of them +12%); other orders of the same instructions (no change).
+// (550 instead of 540); a cubic on the FMA pipe for a quarter of the exponentials
+// (+2%, for half of them +12%); other orders of the same instructions (no change);
+// eight more warps that write a block's rows out (no change).
 //
-// 8192 tokens, 32 q and 8 kv heads of 128, bf16: 527 us, 1.04 PFLOP/s, with the
-// clock at 1.7 GHz under the power limit; 445 us for a single pass.
+// 8192 tokens, 32 q and 8 kv heads of 128, bf16: 522 us, 1.05 PFLOP/s, with the
+// clock at 1.65 to 1.7 GHz under the power limit.
 #include <atomic>
 
 #include "rkv_gqa.cuh"
@@ -952,9 +953,14 @@ static rkv_status launch(const Params& p, const CUtensorMap& map, const CUtensor
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= kMaxDevicesCached || !ready[dev].load(std::memory_order_acquire)) {
-    const cudaError_t e =
+    cudaError_t e =
         cudaFuncSetAttribute(prefill_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<D>::kTotal);
+    cudaFuncAttributes built;
+    if (e == cudaSuccess) e = cudaFuncGetAttributes(&built, prefill_kernel<T, D>);
     if (e != cudaSuccess) return fail(RKV_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
+    // taking more registers than the launch has would wait for ever
+    if (3 * built.numRegs < 2 * kSoftmaxRegs + kOtherRegs)
+      return fail(RKV_ERR_CUDA, "%s: built with %d registers a thread, which the register split exceeds", what, built.numRegs);
     if (dev >= 0 && dev < kMaxDevicesCached) ready[dev].store(true, std::memory_order_release);
   }
   cudaLaunchAttribute attr;
