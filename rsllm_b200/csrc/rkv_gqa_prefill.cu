@@ -72,6 +72,7 @@ constexpr int kBlockRows = 2 * kM;
 constexpr int kBlockCost = 192;    // what a block costs beside its rows, in rows
 constexpr int kRunCost = 8 * kN + kBlockCost;  // no more CTAs than have this much, or a block each
 constexpr int kJobs = 4;           // blocks handed out ahead
+constexpr int kWhole = 8;          // steps that are not shared out: with page tables no wider, no join is launched
 constexpr uint32_t kTmemCols = 512;
 // The launch has 168 registers a thread; the two softmax warpgroups take what the
 // third does without.  (Calls that are not inlined do not go with it: ptxas
@@ -257,12 +258,12 @@ struct Blocks {
     return end(i) > begin(i) ? (end(i) + kN - 1) / kN - begin(i) / kN : 0;
   }
 };
-// Where a cut at `at` of a block's cost goes: its step.  Blocks of up to 8 steps
-// stay whole, longer ones are not cut within 4 of their ends.
+// Where a cut at `at` of a block's cost goes: its step.  Blocks of up to kWhole
+// steps stay whole, longer ones are not cut within 4 of their ends.
 __device__ __forceinline__ int cut_step(long long at, long long cost, int steps) {
   if (at <= 0) return 0;
   if (at >= cost) return steps;
-  if (steps <= 8) return 2 * at >= cost ? steps : 0;
+  if (steps <= kWhole) return 2 * at >= cost ? steps : 0;
   const int k = (int)(at * steps / cost);
   return k < 4 ? 0 : steps - k < 4 ? steps : k;
 }
@@ -974,7 +975,7 @@ static rkv_status launch(const Params& p, const CUtensorMap& map, const CUtensor
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
   cudaError_t e = cudaLaunchKernelEx(&cfg, prefill_kernel<T, D>, p, map, qmap);
-  if (e == cudaSuccess) {
+  if (e == cudaSuccess && p.pt_stride > kWhole) {
     cfg.gridDim = dim3(kGrid, kBlockRows / 32);
     cfg.blockDim = dim3(kJoinThreads);
     cfg.dynamicSmemBytes = 0;

@@ -111,6 +111,7 @@ class GqaKvPool:
         self._s = status.data_ptr()
         self._prefill_ws = self.lib.rkv_gqa_prefill_workspace_bytes(self._v)
         self._decode_ws = {}  # bytes by number of q heads: they do not grow with the sequences
+        self._kept = {}  # workspaces by stream
         self._scale = 1.0 / math.sqrt(self.head_dim)
 
     # -- status ---------------------------------------------------------------
@@ -151,26 +152,34 @@ class GqaKvPool:
         stride = page_table.shape[1]
         return self._need(page_table, torch.int32, "page_table", (n_seq, stride)), stride
 
-    def _empty(self, shape, dtype: torch.dtype, stream) -> torch.Tensor:
-        """Memory made for a call belongs to the stream that the call runs on."""
-        if stream is None:
-            return torch.empty(shape, dtype=dtype, device=self.device)
-        with torch.cuda.stream(stream):
-            return torch.empty(shape, dtype=dtype, device=self.device)
-
-    def _out(self, out: torch.Tensor | None, shape, name: str, stream) -> tuple:
+    def _out(self, out: torch.Tensor | None, q: torch.Tensor, shape, name: str, stream) -> tuple:
+        """An output like q but contiguous; memory made for a call belongs to the stream that the call runs on."""
         if out is None:
-            out = self._empty(shape, self.dtype, stream)
+            if stream is None:
+                out = torch.empty_like(q, memory_format=torch.contiguous_format)
+            else:
+                with torch.cuda.stream(stream):
+                    out = torch.empty_like(q, memory_format=torch.contiguous_format)
             return out, out.data_ptr()
         return out, self._need(out, self.dtype, name, shape)
 
-    def _workspace(self, workspace: torch.Tensor | None, nbytes: int, stream) -> tuple:
-        if workspace is None:
-            workspace = self._empty(nbytes, torch.uint8, stream)
-        elif workspace.get_device() != self._index or not workspace.is_contiguous() or \
-                workspace.numel() * workspace.element_size() < nbytes:
-            raise ShapeMismatch(f"workspace: expected a contiguous tensor of {nbytes} bytes on {self.device}")
-        return workspace, workspace.data_ptr()
+    def _workspace(self, workspace: torch.Tensor | None, nbytes: int, stream, handle: int) -> torch.Tensor:
+        """The caller's workspace, or one that the pool keeps for the current stream (a call on it comes after the one
+        before); with a stream given, or in a graph's capture, memory of the call's own."""
+        if workspace is not None:
+            if workspace.get_device() != self._index or not workspace.is_contiguous() or \
+                    workspace.numel() * workspace.element_size() < nbytes:
+                raise ShapeMismatch(f"workspace: expected a contiguous tensor of {nbytes} bytes on {self.device}")
+            return workspace
+        if stream is not None:
+            with torch.cuda.stream(stream):
+                return torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+        if torch.cuda.is_current_stream_capturing():
+            return torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+        kept = self._kept.get(handle)
+        if kept is None or kept.numel() < nbytes:
+            kept = self._kept[handle] = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+        return kept
 
     def _stream(self, stream) -> int:
         if stream is not None:
@@ -209,7 +218,7 @@ class GqaKvPool:
             if q_shape[0] != n:
                 raise ShapeMismatch("append: q and k differ in tokens")
             heads = q_shape[1]
-            q_out, op = self._out(q_out, q_shape, "q_out", stream)
+            q_out, op = self._out(q_out, q, q_shape, "q_out", stream)
         check(self.lib.rkv_gqa_append(self._v, layer, kp, k_ts, k_hs, vp, v_ts, v_hs, n, slots,
                                       rotary._p if rotary is not None else 0, posp, qp, q_ts, q_hs, heads, op, self._s,
                                       self._stream(stream)), "append")
@@ -231,11 +240,14 @@ class GqaKvPool:
         cu = self._need(cu_q, torch.int32, "cu_q", (n_seq + 1,))
         table, stride = self._table(page_table, n_seq)
         sink = 0 if sinks is None else self._need(sinks, torch.float32, "sinks", (heads,))
-        ws, wp = self._workspace(workspace, self._prefill_ws, stream)
-        out, op = self._out(out, shape, "out", stream)
+        handle = self._stream(stream)
+        ws = self._workspace(workspace, self._prefill_ws, stream, handle)
+        out, op = self._out(out, q, shape, "out", stream)
         scale = self._scale if softmax_scale is None else softmax_scale
-        check(self.lib.rkv_gqa_prefill(self._v, layer, qp, q_ts, q_hs, n, heads, cu, n_seq, table, stride, lens, window,
-                                       sink, scale, wp, op, self._s, self._stream(stream)), "prefill")
+        rc = self.lib.rkv_gqa_prefill(self._v, layer, qp, q_ts, q_hs, n, heads, cu, n_seq, table, stride, lens, window,
+                                      sink, scale, ws.data_ptr(), op, self._s, handle)
+        if rc:
+            check(rc, "prefill")
         return out
 
     def decode(self, layer: int, q: torch.Tensor, page_table: torch.Tensor, kv_lens: torch.Tensor,
@@ -252,11 +264,14 @@ class GqaKvPool:
         sink = 0 if sinks is None else self._need(sinks, torch.float32, "sinks", (heads,))
         if heads not in self._decode_ws:
             self._decode_ws[heads] = max(0, self.lib.rkv_gqa_decode_workspace_bytes(self._v, n_seq, heads))
-        ws, wp = self._workspace(workspace, self._decode_ws[heads], stream)
-        out, op = self._out(out, shape, "out", stream)
+        handle = self._stream(stream)
+        ws = self._workspace(workspace, self._decode_ws[heads], stream, handle)
+        out, op = self._out(out, q, shape, "out", stream)
         scale = self._scale if softmax_scale is None else softmax_scale
-        check(self.lib.rkv_gqa_decode(self._v, layer, qp, q_ts, q_hs, n_seq, heads, table, stride, lens, window, sink,
-                                      scale, wp, op, self._s, self._stream(stream)), "decode")
+        rc = self.lib.rkv_gqa_decode(self._v, layer, qp, q_ts, q_hs, n_seq, heads, table, stride, lens, window, sink,
+                                     scale, ws.data_ptr(), op, self._s, handle)
+        if rc:
+            check(rc, "decode")
         return out
 
     # -- page moves ------------------------------------------------------------------

@@ -185,6 +185,48 @@ def test_decode_in_a_graph(cuda):
     close(out, *shorter.want(), BF)
 
 
+def test_workspace_is_kept_by_stream_and_fits_every_call(cuda):
+    """Calls of different head counts, on two streams and in a capture, one after another without a workspace given."""
+    a = Batch([1] * 3, [3000, 700, 1], 16, 2, 128, BF, seed=20)
+    b = Batch([1] * 2, [900, 2000], 64, 2, 128, BF, seed=21)
+    pa, pb = GqaKvPool.over(a.cache), GqaKvPool.over(b.cache)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for pool, batch in ((pa, a), (pb, b), (pa, a)):
+        with torch.cuda.stream(side):
+            two = pool.decode(0, batch.q, batch.table, batch.kv_lens)
+        one = pool.decode(0, batch.q, batch.table, batch.kv_lens)
+        torch.cuda.synchronize()
+        assert torch.equal(one, two)
+        close(one, *batch.want(), BF)
+    # another group of q heads on the same cache needs another size
+    small = Batch([1] * 3, [3000, 700, 1], 4, 2, 128, BF, seed=22)
+    small.k, small.v = a.k, a.v
+    close(pa.decode(0, small.q, a.table, a.kv_lens), *small.want(), BF)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        held = pa.decode(0, a.q, a.table, a.kv_lens)
+    eager = pa.decode(0, a.q, a.table, a.kv_lens)
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(held, eager)
+
+
+@pytest.mark.parametrize("rows", [8 * 64 - 1, 8 * 64, 8 * 64 + 1])
+@pytest.mark.parametrize("op", ["prefill", "decode"])
+def test_around_the_widest_table_without_a_join(cuda, rows, op):
+    """Page tables of 8 pages (no join is launched) and of 9, many sequences, so that cuts fall inside them."""
+    n = 70
+    b = Batch([1 if op == "decode" else 5] * n, [rows - i % 40 for i in range(n)], 12, 4, 64, HF, seed=rows)
+    width = (rows + 63) // 64
+    table = b.table[:, :width].contiguous()
+    pool = GqaKvPool.over(b.cache)
+    out = pool.decode(0, b.q, table, b.kv_lens, sinks=b.sinks) if op == "decode" else \
+        pool.prefill(0, b.q, b.cu_q, table, b.kv_lens, sinks=b.sinks)
+    pool.check(op)
+    close(out, *b.want(sinks=True), HF)
+
+
 @pytest.mark.parametrize("op", ["prefill", "decode"])
 def test_bad_pages_and_lengths(cuda, op):
     """A page id outside the cache reads as zero rows and is reported; a length past the page table is cut and
