@@ -131,9 +131,11 @@ struct AppendParams {
 // and the bytes on their way many: a token's slot and positions are loaded while
 // the one before is worked on, so that its rows and its cosines and sines are
 // one trip to memory together.  20011 tokens of 28 + 4 + 4 heads of 128, three
-// axes, f16: 82 us, 4.57 TB/s (101 to 133 us where every thread worked out its heads
+// axes, f16: 76 us, 4.95 TB/s (101 to 133 us where every thread worked out its heads
 // and the axes of its pairs for every token: 67 instead of 41 million instructions).
-constexpr int kAppendThreads = 128, kAhead = 3, kAppendCtas = 6;
+// Heads a thread x CTAs an SM: 3 x 4 and 3 x 5 76 us, 3 x 6 82 (spills), 2 x 8 99,
+// 4 x 4 80, 1 x 12 118.
+constexpr int kAppendThreads = 128, kAhead = 3, kAppendCtas = 4;
 template <int D>
 struct AppendShape {
   static constexpr int kPerRow = D / 16;                    // threads of a row: lanes of one warp
