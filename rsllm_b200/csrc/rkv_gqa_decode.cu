@@ -31,8 +31,8 @@
 //
 // Measured: 64 sequences of 32768 rows, 32 q and 8 kv heads of 128, bf16: 1.255 ms,
 // 6.85 TB/s (a copy, which also writes, reaches 6.47).  One sequence of 131072
-// rows and 2 kv heads: 31.4 us, of which 5 pass before the first page is there
-// and 6 in the join; 256 ragged ones of up to 4096 rows, 4 kv heads of 64, f16: 137
+// rows and 2 kv heads: 30.6 us, of which 5 pass before the first page is there
+// and 5 in the join; 256 ragged ones of up to 4096 rows, 4 kv heads of 64, f16: 137
 // us, 5.8 TB/s.
 #include "rkv_gqa.cuh"
 
@@ -515,12 +515,12 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) decode_kernel(const Para
 
 // Joins the partial softmaxes of the q heads of a shared item: first slot as
 // recorded, then slot 2 c' of every later run c'.  kWarps warps
-// take the parts of a head in turn, four at a time with their loads out together,
-// lanes the head's lanes; the warps' sums are added in order.  Sixteen warps where
-// an item has many parts (one sequence of 131072 rows and 2 kv heads: 148; 14 us
-// with eight warps and one load after another, 6 with sixteen), one where it has
-// a few (256 ragged sequences: 13.5 us with sixteen, whose threads mostly start
-// for nothing).
+// take the parts of a head in turn, several at a time with their loads out
+// together, lanes the head's lanes; the warps' sums are added in order.  Sixteen
+// warps where an item has many parts (one sequence of 131072 rows and 2 kv heads:
+// 148; 14 us with eight warps and one load after another, 5.8 with sixteen and four
+// loads, a microsecond less with ten: one trip for all), one where it has a few (256
+// ragged sequences: 13.5 us with sixteen, whose threads mostly start for nothing).
 constexpr int kJoinThreads = 128;  // with one warp a head: four heads
 template <typename T, int D, int kWarps>
 __global__ void __launch_bounds__(kWarps == 1 ? kJoinThreads : 32 * kWarps) join_kernel(const Params p) {
@@ -536,7 +536,7 @@ __global__ void __launch_bounds__(kWarps == 1 ? kJoinThreads : 32 * kWarps) join
   const int head = (item / p.chunks) * p.group + (item % p.chunks) * kRows + r;
   const int count = join.y - join.x / 2 + 1;
   auto slot = [&](int i) { return (int64_t)(i == 0 ? join.x : 2 * (join.x / 2 + i)); };
-  constexpr int kAhead = 4;
+  constexpr int kAhead = kWarps == 1 ? 4 : 10;
   float o[D / 32] = {};
   float m = -INFINITY, l = 0.f;
   for (int i0 = warp; i0 < count; i0 += kAhead * kWarps) {
