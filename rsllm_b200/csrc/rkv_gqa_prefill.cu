@@ -34,7 +34,8 @@
 // of its own), O0, O1 (head_dim columns each).  S of step j + 2 is issued behind
 // O += P V of step j, so a tile's next logits are there before its warps are
 // done with the last ones, and neither they nor the tensor cores wait for the
-// other's latency.  (With one S buffer of 128 columns a tile the chain softmax
+// other's latency.  (S overwrites the P that the product before it reads: a
+// tile's MMAs come from one thread, and run in its order.)  (With one S buffer of 128 columns a tile the chain softmax
 // -> P -> O -> next S was 3400-4000 clocks a step beside 2400 of MMAs.)  An
 // issuing thread is held up until the tensor cores are nearly done with what it
 // issued, so each tile has a warp of its own for it: one warp for both left
