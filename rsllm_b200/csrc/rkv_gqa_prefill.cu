@@ -24,38 +24,46 @@
 //
 //   warps 0-3, 4-7  softmax of tile 0 and of tile 1, one row a thread: S from
 //                   tensor memory, running maximum and sum, P (in the cache's
-//                   type) back over S; the epilogue
+//                   type) back to it; the epilogue
 //   warps 8, 9      issue S = Q K^T (Q, K in shared memory) and O += P V (P in
 //                   tensor memory, V in shared memory) of tile 0 and of tile 1
 //   warp 10         copies Q, K and V by tensor maps into a ring of stages
 //   warp 11         walks the run and hands out its blocks
 //
-// Tensor memory: two S buffers of 64 columns for each tile (P over the first 32
-// of its own), O0, O1 (head_dim columns each).  S of step j + 2 is issued behind
-// O += P V of step j, so a tile's next logits are there before its warps are
-// done with the last ones, and neither they nor the tensor cores wait for the
-// other's latency.  (S overwrites the P that the product before it reads: a
-// tile's MMAs come from one thread, and run in its order.)  (With one S buffer of 128 columns a tile the chain softmax
-// -> P -> O -> next S was 3400-4000 clocks a step beside 2400 of MMAs.)  An
-// issuing thread is held up until the tensor cores are nearly done with what it
-// issued, so each tile has a warp of its own for it: one warp for both left
-// them idle for the 200-700 clocks of its waits between two batches.
+// Tensor memory of a tile: S of a step (64 columns), P of two steps (32 each), O
+// (head_dim columns).  S of the next step is issued when the softmax warps have
+// loaded the last one into their registers, and is there when they are done with
+// it.  Two MMAs run in the order of their issue only if they have the same
+// accumulator and shape, so whatever is overwritten here has been read behind a
+// barrier: S when the softmax warps say so, P of step j - 2 when S of step j
+// is there (the commit behind S covers the product issued before it by the same
+// thread), O by its own products.
 //
-// What bounds a step of both tiles (1650 to 1750 clocks, head_dim 128): 1280 of
+// An issuing thread is held up until the tensor cores are nearly done with what it
+// issued, so each tile has a warp of its own for it, and what a warp waits for
+// besides is asked for by a lane each, in one instruction: a barrier takes 150 to
+// 250 clocks while the operand reads fill the shared memory.  (One after another
+// they were 350 clocks more a step, and the issuing warp bound the step: 580 us
+// for 8192 tokens.)
+//
+// What bounds a step of both tiles (1750 to 1950 clocks, head_dim 128): 1280 of
 // MMAs -- S with 64 columns reads 6 KB of operands for 32 clocks of products, the
 // shared memory's 128 bytes a clock make it 48 -- and a chain of the softmax
-// warps: 290 for loads, maxima and masks, 930 for 64 exponentials, conversions
-// and sums (1070 when both tiles' warps meet there; 512 each at 16 a clock), and
-// 150 to 250 for every barrier while the operand reads fill the shared memory.
-// Measured and not kept: two sets of softmax warps taking a tile's steps in
-// turn (head_dim 128: 539 us instead of 527 for 8192 tokens; head_dim 64: 5%
-// faster); the tiles' warps handing each other the exponentials by named barriers
-// (550 instead of 540); a cubic on the FMA pipe for a quarter of the exponentials
-// (+2%, for half of them +12%); other orders of the same instructions (no change);
-// eight more warps that write a block's rows out (no change).
+// warps: 150 for the barrier of S, 80 to 110 for loads, 160 to 250 for maxima and
+// masks, 930 for 64 exponentials, conversions and sums (1070 to 1280 when both
+// tiles' warps meet there; 512 each at 16 a clock).
+// Measured and not kept: P over its own S, with two S buffers a tile and a wait for
+// the product that reads P before the S that overwrites it (642 us for 8192 tokens);
+// S issued before the product of the step before it (594: P then waits for that
+// product); one S buffer of 128 columns a tile, 3400-4000 clocks a step beside
+// 2400 of MMAs; two sets of softmax warps taking a tile's steps in turn; the
+// tiles' warps handing each other the exponentials by named barriers; a cubic on
+// the FMA pipe for a quarter of the exponentials (+2%, for half of them +12%);
+// other orders of the same instructions (no change); eight more warps that write
+// a block's rows out (no change).
 //
-// 8192 tokens, 32 q and 8 kv heads of 128, bf16: 522 us, 1.05 PFLOP/s, with the
-// clock at 1.65 to 1.7 GHz under the power limit.
+// 8192 tokens, 32 q and 8 kv heads of 128, bf16: 519 to 550 us, 1.0 to 1.06
+// PFLOP/s, with the clock at 1.65 to 1.7 GHz under the power limit.
 #include <atomic>
 
 #include "rkv_gqa.cuh"
@@ -111,15 +119,16 @@ struct Layout {
   static constexpr int kJob = kRing + kStages * kStage;   // [kJobs] of 64 bytes
   static constexpr int kBars = kJob + 64 * kJobs;
   static constexpr int kBarEmpty = 8 * kStages;   // full[kStages], empty[kStages]
-  static constexpr int kBarS = 16 * kStages;      // S full [2][2]
+  static constexpr int kBarS = 16 * kStages;      // S full [2][2], of even and odd steps
   static constexpr int kBarP = kBarS + 32;        // P full [2][2]
-  static constexpr int kBarPv = kBarP + 32;       // O += P V of a step done [2]
-  static constexpr int kBarO = kBarPv + 16;       // O of a block done [2]
+  static constexpr int kBarPv = kBarP + 32;       // O += P V of a step done [2][2]
+  static constexpr int kBarO = kBarPv + 32;       // O of a block done [2]
   static constexpr int kBarOFree = kBarO + 16;    // and read [2]
   static constexpr int kBarQ = kBarOFree + 16;    // Q full, Q free
   static constexpr int kBarJob = kBarQ + 16;      // job full[kJobs], free[kJobs]
   static constexpr int kBarDrain = kBarJob + 16 * kJobs;  // [2]
-  static constexpr int kMisc = kBars + kBarDrain + 16;    // TMEM address, abort flag, start of the run
+  static constexpr int kBarSFree = kBarDrain + 16;        // S read [2]
+  static constexpr int kMisc = kBars + kBarSFree + 16;    // TMEM address, abort flag, start of the run
   static constexpr int kScan = kMisc + 32;                // sums of the warps: costs, blocks
   static constexpr int kTotal = kScan + 12 * (kThreads / 32) + 1024;  // slack for the 1024-byte alignment
 };
@@ -193,8 +202,8 @@ __device__ __forceinline__ unsigned long long pk2(uint32_t lo, uint32_t hi) {
 }
 __device__ __forceinline__ unsigned long long dup2(float x) { return pk2(__float_as_uint(x), __float_as_uint(x)); }
 
-// The weights 2^(x scale - m) of a row's 64 logits, stored over S as P in the
-// cache's type; returns their sum.  (A cubic on the FMA pipe in place of a
+// The weights 2^(x scale - m) of a row's 64 logits, stored as P in the cache's
+// type; returns their sum.  (A cubic on the FMA pipe in place of a
 // quarter to a half of the exponentials made the 8192-token prompt 2 to 12%
 // slower: its 7 instructions a pair cost more than the exponential unit has
 // to spare.)
@@ -305,12 +314,13 @@ prefill_kernel(const Params p, const __grid_constant__ CUtensorMap map, const __
     for (int i = 0; i < 4; ++i) {
       mbar_init(bars + L::kBarS + 8 * i, 1);
       mbar_init(bars + L::kBarP + 8 * i, 128);
+      mbar_init(bars + L::kBarPv + 8 * i, 1);
     }
     for (int t = 0; t < 2; ++t) {
-      mbar_init(bars + L::kBarPv + 8 * t, 1);
       mbar_init(bars + L::kBarO + 8 * t, 1);
       mbar_init(bars + L::kBarOFree + 8 * t, 4);  // warps of a tile
       mbar_init(bars + L::kBarDrain + 8 * t, 1);
+      mbar_init(bars + L::kBarSFree + 8 * t, 4);
     }
     mbar_init(bars + L::kBarQ, 1);
     mbar_init(bars + L::kBarQ + 8, 2);
@@ -511,10 +521,9 @@ prefill_kernel(const Params p, const __grid_constant__ CUtensorMap map, const __
       struct Place {  // in the ring: stage and parity of its phase
         int st;
         uint32_t ph;
-        __device__ __forceinline__ void skip(int n) {
-          st += n;
-          if (st >= L::kStages) {
-            st -= L::kStages;
+        __device__ __forceinline__ void next() {
+          if (++st == L::kStages) {
+            st = 0;
             ph ^= 1u;
           }
         }
@@ -525,15 +534,14 @@ prefill_kernel(const Params p, const __grid_constant__ CUtensorMap map, const __
       // S of the tile's step n (one lane)
       auto qk = [&](const Place& at, int n) {
         const uint64_t kd = kd0 + (uint64_t)((at.st * L::kStage) >> 4);
-        const uint32_t d = ts + (n & 1) * 64;
 #pragma unroll
         for (int k = 0; k < D / 16; ++k)
-          mma_ss(d, qd + (uint64_t)(((k >> 2) * L::kQCol + (k & 3) * 32) >> 4),
+          mma_ss(ts, qd + (uint64_t)(((k >> 2) * L::kQCol + (k & 3) * 32) >> 4),
                  kd + (uint64_t)(((k >> 2) * L::kCol + (k & 3) * 32) >> 4), kIdescS, k > 0);
         mma_commit(bars + L::kBarS + 16 * t + 8 * (n & 1));
         mma_commit(bars + L::kBarEmpty + 8 * at.st);
       };
-      Place kp = {0, 0u};
+      Place at = {0, 0u};
       int n = 0;       // steps of this tile so far: of step j of a job, n + j
       int n_q = 0;     // jobs with steps
       int n_o = 0;     // of which this tile had some
@@ -544,71 +552,66 @@ prefill_kernel(const Params p, const __grid_constant__ CUtensorMap map, const __
         const int tiles = w.tokens > p.tile_tokens ? 2 : 1;
         const int steps = t == tiles - 1 ? w.steps : t < tiles ? w.steps0 : 0;
         ok = __all_sync(0xffffffffu, mbar_wait(bars + L::kBarQ, n_q & 1, abort_flag));
-        // K and V lie in the ring in the order K0 K1 V0 K2 V1 ... V of the last step
-        Place vp = kp;
-        vp.skip(w.steps > 1 ? 2 : 1);
         if (steps == 0 && elect_one()) mbar_arrive(bars + L::kBarQ + 8);
         __syncwarp();
-        for (int j = 0; ok && j < 2 && j < w.steps; ++j) {  // places 0 and 1
-          ok = full(kp);
-          if (!ok) break;
-          if (elect_one()) {
-            if (j < steps) qk(kp, n + j);
-            else mbar_arrive(bars + L::kBarEmpty + 8 * kp.st);
-            if (j == steps - 1) mma_commit(bars + L::kBarQ + 8);
+        // K and V lie in the ring in the order K0 K1 V0 K2 V1 ... V of the last step
+        ok = ok && full(at);
+        for (int j = -1; ok && j < w.steps; ++j) {
+          if (j + 1 < w.steps) {  // S of step j + 1, once the softmax warps have read the one before it
+            if (j + 1 < steps && n + j >= 0) {
+              ok = __all_sync(0xffffffffu, mbar_wait(bars + L::kBarSFree + 8 * t, (n + j) & 1, abort_flag));
+              if (!ok) break;
+              tc_fence_after();
+            }
+            if (elect_one()) {
+              if (j + 1 < steps) qk(at, n + j + 1);
+              else mbar_arrive(bars + L::kBarEmpty + 8 * at.st);  // the other tile's steps
+              if (j + 1 == steps - 1) mma_commit(bars + L::kBarQ + 8);  // Q may be overwritten
+            }
+            __syncwarp();
+            at.next();
           }
-          __syncwarp();
-          kp.skip(j + 1);  // to 1, then 3
-        }
-        if (w.steps == 1) kp.skip(1);  // past V0
-        for (int j = 0; ok && j < w.steps; ++j) {
-          ok = full(vp) && (j + 2 >= w.steps || full(kp));
+          if (j < 0) {
+            if (w.steps > 1) ok = full(at);
+            continue;
+          }
+          // a barrier a lane: V of this step, K of the one after next, P of this step, the O of the block before read
+          const Place v = at;
+          at.next();
+          uint32_t bar = bars + 8 * v.st, ph = v.ph;
+          if ((lane & 3) == 1 && j + 2 < w.steps) bar = bars + 8 * at.st, ph = at.ph;
+          if ((lane & 3) == 2 && j < steps) bar = bars + L::kBarP + 16 * t + 8 * ((n + j) & 1), ph = ((n + j) >> 1) & 1;
+          if ((lane & 3) == 3 && j == 0 && steps > 0 && n_o > 0) bar = bars + L::kBarOFree + 8 * t, ph = (n_o - 1) & 1;
+          ok = __all_sync(0xffffffffu, mbar_wait(bar, ph, abort_flag));
           if (!ok) break;
+          tc_fence_after();
           const int past = w.len - (w.step0 + j) * kN;  // first row past the sequence's end: zeros there (both warps do it)
           if (past < kN) {
             for (int i = lane; i < (kN - past) * (D / 8); i += 32) {
               const int r = past + i / (D / 8), c = i % (D / 8);
-              *reinterpret_cast<uint4*>(smem + L::kRing + vp.st * L::kStage + (c >> 3) * L::kCol + r * 128 +
+              *reinterpret_cast<uint4*>(smem + L::kRing + v.st * L::kStage + (c >> 3) * L::kCol + r * 128 +
                                         (((c & 7) ^ (r & 7)) << 4)) = make_uint4(0, 0, 0, 0);
             }
             fence_proxy_async();
             __syncwarp();
           }
-          if (j < steps) {
-            // the softmax warps have read the O before this one
-            if (j == 0 && n_o > 0)
-              ok = __all_sync(0xffffffffu, mbar_wait(bars + L::kBarOFree + 8 * t, (n_o - 1) & 1, abort_flag));
-            ok = ok && __all_sync(0xffffffffu, mbar_wait(bars + L::kBarP + 16 * t + 8 * ((n + j) & 1),
-                                                         ((n + j) >> 1) & 1, abort_flag));
-            if (!ok) break;
-            tc_fence_after();
-          }
           if (elect_one()) {
             if (j < steps) {
-              const uint64_t vd = vd0 + (uint64_t)((vp.st * L::kStage) >> 4);
-              const uint32_t pa = ts + ((n + j) & 1) * 64;
+              const uint64_t vd = vd0 + (uint64_t)((v.st * L::kStage) >> 4);
+              const uint32_t pa = ts + kN + ((n + j) & 1) * (kN / 2);
 #pragma unroll
               for (int k = 0; k < kN / 16; ++k)
                 mma_ts(to, pa + 8 * k, vd + (uint64_t)((k * 2048) >> 4), kIdescO, (j > 0 || k > 0) ? 1u : 0u);
-              mma_commit(bars + L::kBarPv + 8 * t);
+              mma_commit(bars + L::kBarPv + 16 * t + 8 * ((n + j) & 1));
               if (j == steps - 1) mma_commit(bars + L::kBarO + 8 * t);
-              mma_commit(bars + L::kBarEmpty + 8 * vp.st);
-            } else {  // the other tile's steps
-              mbar_arrive(bars + L::kBarEmpty + 8 * vp.st);
-            }
-            if (j + 2 < steps) {
-              qk(kp, n + j + 2);
-              if (j + 2 == steps - 1) mma_commit(bars + L::kBarQ + 8);  // Q may be overwritten
-            } else if (j + 2 < w.steps) {
-              mbar_arrive(bars + L::kBarEmpty + 8 * kp.st);
+              mma_commit(bars + L::kBarEmpty + 8 * v.st);
+            } else {
+              mbar_arrive(bars + L::kBarEmpty + 8 * v.st);
             }
           }
           __syncwarp();
-          vp.skip(j + 2 < w.steps ? 2 : 1);
-          if (j + 2 < w.steps) kp.skip(j + 3 < w.steps ? 2 : 1);
         }
         if (!ok) break;
-        kp = vp;  // past the last V
         n += steps;
         n_q += 1;
         n_o += steps > 0;
@@ -719,19 +722,21 @@ prefill_kernel(const Params p, const __grid_constant__ CUtensorMap map, const __
       const int pos_max = pos_min + p.tile_tokens - 1;
       float m = -INFINITY;  // exponent reference of l
       float l = 0.f;        // sum of the weights
-      bool ready = false;
       for (int j = 0; j < steps; ++j) {
         const int b = (n + j) & 1;
-        const uint32_t ts = ts0 + 64 * b;
-        if (!__all_sync(0xffffffffu, ready || mbar_wait(bars + L::kBarS + 16 * t + 8 * b, ((n + j) >> 1) & 1, abort_flag))) {
+        const uint32_t ts = ts0 + kN + (kN / 2) * b;  // P
+        if (!__all_sync(0xffffffffu, mbar_wait(bars + L::kBarS + 16 * t + 8 * b, ((n + j) >> 1) & 1, abort_flag))) {
           ok = false;
           break;
         }
         tc_fence_after();
         uint32_t x[kN];
 #pragma unroll
-        for (int i = 0; i < kN; i += 32) tmem_ld32(ts + i, x + i);
+        for (int i = 0; i < kN; i += 32) tmem_ld32(ts0 + i, x + i);
         tmem_wait_ld();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bars + L::kBarSFree + 8 * t);  // S may be overwritten
         const int key0 = row0 + j * kN;
         if (key0 + kN - 1 > pos_min || (p.window > 0 && key0 <= pos_max - p.window)) {
           const int last = row_token - key0, first = p.window > 0 ? last - p.window : -1;
@@ -757,9 +762,9 @@ prefill_kernel(const Params p, const __grid_constant__ CUtensorMap map, const __
           m = up ? top : m;
           l *= a;
           if (j > 0) {
-            // O holds the steps up to j - 1 once their MMAs are done: S of this step was issued behind step j - 2's,
-            // and step j's wait for this warp, so the barrier is in that phase or just past it
-            if (!__all_sync(0xffffffffu, mbar_wait(bars + L::kBarPv + 8 * t, (n + j - 1) & 1, abort_flag))) {
+            // O holds the steps up to j - 1 once their MMAs are done.  The product before on that barrier, of step j - 3,
+            // was done before P of step j - 1 was written, and the one after waits for this warp's P of step j + 1.
+            if (!__all_sync(0xffffffffu, mbar_wait(bars + L::kBarPv + 16 * t + 8 * (1 - b), ((n + j - 1) >> 1) & 1, abort_flag))) {
               ok = false;
               break;
             }
@@ -775,10 +780,6 @@ prefill_kernel(const Params p, const __grid_constant__ CUtensorMap map, const __
             }
           }
         }
-        // Asked here, the next S's barrier answers behind the exponentials.  With head_dim 64 that is 4% (360 to 345
-        // us for 8 x 64-256 tokens behind 8192 rows); with 128, S is not there yet and it costs 2%.
-        if constexpr (D == 64)
-          ready = j + 1 < steps && mbar_test(bars + L::kBarS + 16 * t + 8 * (1 - b), ((n + j + 1) >> 1) & 1);
         const unsigned long long n2 = dup2(m == -INFINITY ? 0.f : -m);  // nothing seen yet: weights 0
         l += weights<T>(x, ts, c2, n2);
         tmem_wait_st();

@@ -1,0 +1,25 @@
+"""More of the grouped-head paged cache on the GPU: what only shows over many steps, at the ends of the arguments'
+ranges, with values that are not finite, and from several threads."""
+import pytest
+import torch
+
+from rsllm_b200 import GqaKvPool
+from tests.gqa_cases import Batch, close
+
+pytestmark = pytest.mark.gpu
+
+BF, HF = torch.bfloat16, torch.float16
+
+
+# ---------------------------------------------------------- tensor memory
+@pytest.mark.parametrize("d,dtype", [(128, BF), (64, HF)])
+def test_prefill_repeats_itself(cuda, d, dtype):
+    """Every run gives the same bits: the buffers of S, P and O in tensor memory are never overwritten before they are
+    read, whatever else the tensor cores are at.  The logits grow along the sequences, so that O is rescaled too."""
+    b = Batch([1500, 700, 3], [1500, 2700, 4000], 8, 2, d, dtype, seed=30, q_scale=8.0)
+    pool = GqaKvPool.over(b.cache)
+    first = pool.prefill(0, b.q, b.cu_q, b.table, b.kv_lens)
+    close(first, *b.want(), dtype)
+    for _ in range(40):
+        assert torch.equal(pool.prefill(0, b.q, b.cu_q, b.table, b.kv_lens), first)
+    pool.check("prefill")
