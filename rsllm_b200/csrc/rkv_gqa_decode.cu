@@ -35,6 +35,7 @@
 // and 5 in the join; 256 ragged ones of up to 4096 rows, 4 kv heads of 64, f16: 137
 // us, 5.8 TB/s.
 #include "rkv_gqa.cuh"
+#include "rkv_gqa_plan.h"
 
 #include <atomic>
 
@@ -239,7 +240,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) decode_kernel(const Para
     const int rows_total = (int)row_base(p.cache, p.cache.n_layers, 0, 0, 0);  // out of range: zero rows
     int n = 0;
     bool ok = true;
-    for (; left > 0 && ok; ++s) {
+    for (; left > 0 && ok && s < p.n_seq; ++s) {
       const Seen see = seen_rows(p, s);
       const int pages = see.pages();
       if (pages == 0) continue;
@@ -297,7 +298,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) decode_kernel(const Para
   const int rows = min(p.group, kRows);
   int n = 0, segment = 0;
   bool ok = true;
-  for (; left > 0 && ok; ++s) {
+  for (; left > 0 && ok && s < p.n_seq; ++s) {
     const Seen see = seen_rows(p, s);
     const int pages = see.pages();
     if (pages == 0) continue;
@@ -694,7 +695,7 @@ extern "C" rkv_status rkv_gqa_decode(const rkv_gqa_view* cache, int32_t layer, c
   p.page_table = page_table;
   p.pt_stride = pt_stride;
   p.kv_lens = kv_lens;
-  p.window = window;
+  p.window = window_of(window, pt_stride);
   p.sinks = sinks;
   p.scale_log2 = (float)((double)softmax_scale * 1.4426950408889634);
   const int64_t rows = p.group < kRows ? p.group : kRows;

@@ -67,21 +67,20 @@
 #include <atomic>
 
 #include "rkv_gqa.cuh"
+#include "rkv_gqa_plan.h"
 
 namespace rkv {
 namespace gqa {
 namespace pre {
 
 constexpr int kM = 128;        // q rows of a tile
-constexpr int kN = kPage;      // key rows of a step
+static_assert(kN == kPage, "a step is a page");
 constexpr int kMmaWarp = 8, kLoadWarp = 10, kPlanWarp = 11;
 constexpr int kThreads = 384;
 constexpr int kGrid = 148;         // one CTA an SM
 constexpr int kBlockRows = 2 * kM;
-constexpr int kBlockCost = 192;    // what a block costs beside its rows, in rows
 constexpr int kRunCost = 8 * kN + kBlockCost;  // no more CTAs than have this much, or a block each
 constexpr int kJobs = 4;           // blocks handed out ahead
-constexpr int kWhole = 8;          // steps that are not shared out: with page tables no wider, no join is launched
 constexpr uint32_t kTmemCols = 512;
 // The launch has 168 registers a thread; the two softmax warpgroups take what the
 // third does without.  (Calls that are not inlined do not go with it: ptxas
@@ -233,49 +232,11 @@ __device__ __forceinline__ int2 new_tokens(const Params& p, int s) {
   return make_int2(a, min(max(__ldg(p.cu_q + s + 1), a), p.n_tokens));
 }
 
-// A sequence's blocks for one kv head.  Block i has the tokens [i span, (i + 1)
-// span) and sees the rows [begin(i), end(i)); it weighs as many and kBlockCost.
-struct Blocks {
-  int token, tokens, len, pos, span, window, count;
-  __device__ __forceinline__ void init(const Params& p, int s) {
-    const int2 t = new_tokens(p, s);
-    token = t.x;
-    tokens = t.y - t.x;
-    len = min(max(__ldg(p.kv_lens + s), 0), (int)p.pt_stride * kPage);
-    pos = len - tokens;  // position of the first token, may be negative
-    span = 2 * p.tile_tokens;
-    window = p.window;
-    count = (tokens + span - 1) / span;
-  }
-  __device__ __forceinline__ int end(int i) const { return max(0, pos + min(tokens, (i + 1) * span)); }
-  __device__ __forceinline__ int begin(int i) const { return window > 0 ? max(0, pos + i * span - window + 1) : 0; }
-  __device__ __forceinline__ long long cost(int i) const { return kBlockCost + end(i) - min(begin(i), end(i)); }
-  // sum over i < n of max(0, a + i span)
-  __device__ __forceinline__ long long ramp(long long n, long long a) const {
-    const long long i0 = a > 0 ? 0 : (-a) / span + 1;  // the first above zero
-    if (i0 >= n) return 0;
-    return (n - i0) * a + span * (n * (n - 1) / 2 - i0 * (i0 - 1) / 2);
-  }
-  // cost of the blocks before n
-  __device__ __forceinline__ long long before(int n) const {
-    long long c = (long long)n * kBlockCost + ramp(n, (long long)pos + span);
-    if (window > 0) c -= ramp(n, (long long)pos - window + 1);
-    if (n == count && n > 0) c -= (long long)pos + (long long)n * span - len;  // the last one may be short
-    return c;
-  }
-  __device__ __forceinline__ int first_step(int i) const { return begin(i) / kN; }
-  __device__ __forceinline__ int steps(int i) const {
-    return end(i) > begin(i) ? (end(i) + kN - 1) / kN - begin(i) / kN : 0;
-  }
-};
-// Where a cut at `at` of a block's cost goes: its step.  Blocks of up to kWhole
-// steps stay whole, longer ones are not cut within 4 of their ends.
-__device__ __forceinline__ int cut_step(long long at, long long cost, int steps) {
-  if (at <= 0) return 0;
-  if (at >= cost) return steps;
-  if (steps <= kWhole) return 2 * at >= cost ? steps : 0;
-  const int k = (int)(at * steps / cost);
-  return k < 4 ? 0 : steps - k < 4 ? steps : k;
+__device__ __forceinline__ Blocks blocks_of(const Params& p, int s) {
+  const int2 t = new_tokens(p, s);
+  Blocks b;
+  b.init(t.x, t.y - t.x, min(max(__ldg(p.kv_lens + s), 0), (int)p.pt_stride * kPage), p.tile_tokens, p.window);
+  return b;
 }
 
 // A block, or a part of its steps, as handed to the warps.
@@ -357,8 +318,7 @@ prefill_kernel(const Params p, const __grid_constant__ CUtensorMap map, const __
     const int s_begin = min(tid * per, p.n_seq), s_end = min(s_begin + per, p.n_seq);
     long long mine = 0, blocks = 0;
     for (int s = s_begin; s < s_end; ++s) {
-      Blocks b;
-      b.init(p, s);
+      const Blocks b = blocks_of(p, s);
       mine += b.before(b.count) * p.cache.n_kv_heads;
       blocks += (long long)b.count * p.cache.n_kv_heads;
       if (blockIdx.x == 0 && (b.len != __ldg(p.kv_lens + s) || b.token != __ldg(p.cu_q + s) ||
@@ -394,8 +354,7 @@ prefill_kernel(const Params p, const __grid_constant__ CUtensorMap map, const __
     long long at = upto - mine;
     if (u0 < u1 && u0 >= at && u0 < upto) {
       for (int s = s_begin; s < s_end; ++s) {
-        Blocks b;
-        b.init(p, s);
+        const Blocks b = blocks_of(p, s);
         const long long n = b.before(b.count) * p.cache.n_kv_heads;
         if (u0 < at + n) {
           *start_seq = s;
@@ -451,9 +410,8 @@ prefill_kernel(const Params p, const __grid_constant__ CUtensorMap map, const __
       if (left > 0) {
         int s = *start_seq;
         long long off = *start_off;
-        for (; left > 0 && ok; ++s, off = 0) {
-          Blocks b;
-          b.init(p, s);
+        for (; left > 0 && ok && s < p.n_seq; ++s, off = 0) {
+          const Blocks b = blocks_of(p, s);
           const long long per_head = b.before(b.count);
           if (per_head == 0) continue;
           int head = 0;
@@ -739,7 +697,7 @@ prefill_kernel(const Params p, const __grid_constant__ CUtensorMap map, const __
         if (lane == 0) mbar_arrive(bars + L::kBarSFree + 8 * t);  // S may be overwritten
         const int key0 = row0 + j * kN;
         if (key0 + kN - 1 > pos_min || (p.window > 0 && key0 <= pos_max - p.window)) {
-          const int last = row_token - key0, first = p.window > 0 ? last - p.window : -1;
+          const int last = row_token - key0, first = p.window > 0 ? max(last, -1) - p.window : -1;
 #pragma unroll
           for (int i = 0; i < kN; ++i)
             if (i > last || i <= first) x[i] = 0xff800000u;  // -inf
@@ -1037,7 +995,7 @@ extern "C" rkv_status rkv_gqa_prefill(const rkv_gqa_view* cache, int32_t layer, 
   p.page_table = page_table;
   p.pt_stride = pt_stride;
   p.kv_lens = kv_lens;
-  p.window = window;
+  p.window = window_of(window, pt_stride);
   p.sinks = sinks;
   p.scale_log2 = (float)((double)softmax_scale * 1.4426950408889634);
   p.part_o = static_cast<float*>(workspace);

@@ -23,3 +23,21 @@ def test_prefill_repeats_itself(cuda, d, dtype):
     for _ in range(40):
         assert torch.equal(pool.prefill(0, b.q, b.cu_q, b.table, b.kv_lens), first)
     pool.check("prefill")
+
+
+# ------------------------------------------------------- windows without end
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 30, 2 ** 30, 640, 639])
+@pytest.mark.parametrize("op", ["prefill", "decode"])
+def test_widest_windows(cuda, op, window):
+    """The largest int as "no window", with fewer rows than new tokens among the sequences; and windows of just the
+    rows that the page tables hold (10 pages) and one fewer."""
+    q_lens, kv_lens = ([50, 300, 4, 70], [20, 0, 1, 576]) if op == "prefill" else ([1] * 4, [576, 0, 1, 130])
+    b = Batch(q_lens, kv_lens, 8, 2, 128, BF, seed=31)
+    assert b.table.shape[1] == 10
+    pool = GqaKvPool.over(b.cache)
+    if op == "prefill":
+        out = pool.prefill(0, b.q, b.cu_q, b.table, b.kv_lens, window=window)
+    else:
+        out = pool.decode(0, b.q, b.table, b.kv_lens, window=window)
+    pool.check(op)
+    close(out, *b.want(window=window), BF)
