@@ -69,6 +69,7 @@ struct Params {
   float* part_o;   // [2 * kGrid][rows][head_dim], rows = min(group, 16)
   float* part_ml;  // [2 * kGrid][rows][2]
   int by_item;     // joins has an entry for each item (fewer than the runs), else for each run, whose last item it is
+  int runs;        // CTAs of the launch
   int4* joins;     // [kGrid]: first slot of a shared item (-1: none), last run, sequence, and kv head and chunk
   uint16_t* out;
   uint32_t* status;
@@ -532,7 +533,9 @@ __global__ void __launch_bounds__(kWarps == 1 ? kJoinThreads : 32 * kWarps) join
   const int warp = kWarps == 1 ? 0 : threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t s = join.z;
   const int item = join.w, r = kWarps == 1 ? blockIdx.y * (kJoinThreads / 32) + (threadIdx.x >> 5) : blockIdx.y;
-  if (join.x < 0 || r >= min(kRows, p.group - (item % p.chunks) * kRows)) return;
+  if (!join_holds(join.x, join.y, join.z, join.w, p.runs, p.n_seq, p.cache.n_kv_heads * p.chunks) ||
+      r >= min(kRows, p.group - (item % p.chunks) * kRows))
+    return;
   const int rows = min(p.group, kRows);
   const int head = (item / p.chunks) * p.group + (item % p.chunks) * kRows + r;
   const int count = join.y - join.x / 2 + 1;
@@ -621,6 +624,7 @@ static rkv_status launch(Params p, const CUtensorMap& map, cudaStream_t s, const
   const int64_t units = (int64_t)p.n_seq * p.cache.n_kv_heads * p.chunks * p.pt_stride;
   const unsigned grid = (unsigned)(units < kGrid ? units : kGrid);
   const int64_t items = (int64_t)p.n_seq * p.cache.n_kv_heads * p.chunks;
+  p.runs = (int)grid;
   p.by_item = grid > 8 * items;  // more than eight parts an item, were they alike
   cfg.gridDim = dim3(grid);
   cfg.blockDim = dim3(kThreads);

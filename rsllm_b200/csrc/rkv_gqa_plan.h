@@ -1,6 +1,7 @@
-// rkv_gqa_plan.h -- how the prefill attention of the grouped-head cache divides
-// its work: the blocks of a sequence, what they weigh, where they may be cut.
-// Plain arithmetic, the same on the device and on the host.
+// rkv_gqa_plan.h -- how the attentions of the grouped-head cache divide their
+// work: the blocks of a prefill's sequence, what they weigh, where they may be
+// cut; what decode's join takes.  Plain arithmetic, the same on the device and
+// on the host.
 #pragma once
 #include <stdint.h>
 
@@ -74,5 +75,15 @@ RKV_PLAN_FN int cut_step(long long at, long long cost, int steps) {
 }
 
 }  // namespace pre
+
+namespace dec {
+
+// Whether an entry of the join's list can be followed: its first slot, the last run, the sequence and the item of it.
+// A launch that gave up (a wait that ran out) leaves entries unwritten, with whatever the workspace held.
+RKV_PLAN_FN bool join_holds(int slot, int last, int seq, int item, int runs, int n_seq, int items) {
+  return slot >= 0 && slot / 2 <= last && last < runs && seq >= 0 && seq < n_seq && item >= 0 && item < items;
+}
+
+}  // namespace dec
 }  // namespace gqa
 }  // namespace rkv

@@ -1,5 +1,5 @@
-"""How the prefill attention of the grouped-head cache divides its work: the arithmetic that the kernel compiles,
-compiled for the host and held to the definition of what a token sees."""
+"""How the attentions of the grouped-head cache divide their work: the arithmetic that the kernels compile, compiled
+for the host and held to the definition of what a token sees."""
 import ctypes
 import random
 import shutil
@@ -14,6 +14,7 @@ INT_MAX = 2 ** 31 - 1
 WRAPPER = """
 #include "rkv_gqa_plan.h"
 using namespace rkv::gqa;
+namespace dec = rkv::gqa::dec;
 using namespace rkv::gqa::pre;
 static Blocks make(int tokens, int len, int tile, int window) {
   Blocks b;
@@ -29,6 +30,9 @@ void block(int tokens, int len, int tile, int window, int i, long long* out) {
   out[5] = b.before(i), out[6] = b.before(i + 1);
 }
 int window(int w, long long pt_stride) { return window_of(w, pt_stride); }
+int joins(int slot, int last, int seq, int item, int runs, int n_seq, int items) {
+  return dec::join_holds(slot, last, seq, item, runs, n_seq, items);
+}
 int cut(long long at, long long cost, int steps) { return cut_step(at, cost, steps); }
 }
 """
@@ -103,3 +107,21 @@ def test_a_window_as_wide_as_the_tables_is_none(plan):
     for stride in (1, 9, 33554431):
         for w in (0, 1, 63, 64, 65, 575, 576, 577, 33554431 * 64 - 1, 33554431 * 64, INT_MAX):
             assert plan.window(w, stride) == (w if w < stride * 64 else 0)
+
+
+def test_join_entries_that_cannot_be_followed(plan):
+    """Entries that a launch which gave up never wrote hold anything: none may lead the join out of its tables."""
+    runs, n_seq, items = 296, 3, 8
+    for slot, last, seq, item in [(0, 0, 0, 0), (1, 0, 2, 7), (591, 295, 0, 3), (0, 295, 2, 0)]:
+        assert plan.joins(slot, last, seq, item, runs, n_seq, items)
+    for slot, last, seq, item in [(-1, 0, 0, 0), (592, 296, 0, 0), (2, 0, 0, 0), (0, 296, 0, 0), (0, -1, 0, 0),
+                                  (0, 5, 3, 0), (0, 5, -1, 0), (0, 5, 0, 8), (0, 5, 0, -1), (INT_MAX, INT_MAX, 0, 0),
+                                  (-1, -1, -1, -1), (0x7f7f7f7f,) * 4, (0, 5, INT_MAX, 0)]:
+        assert not plan.joins(slot, last, seq, item, runs, n_seq, items)
+    r = random.Random(2)
+    for _ in range(20000):
+        e = [r.randint(-2 ** 31, 2 ** 31 - 1) if r.random() < 0.5 else r.randint(-3, 700) for _ in range(4)]
+        if plan.joins(*e, runs, n_seq, items):  # every slot that the join reads, and the row it writes, exists
+            first = e[0] // 2
+            assert all(0 <= s < 2 * runs for s in (e[0], 2 * first, 2 * e[1])) and e[1] - first + 1 <= runs
+            assert 0 <= e[2] < n_seq and 0 <= e[3] < items
