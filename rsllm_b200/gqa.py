@@ -9,6 +9,7 @@ cache; ``GqaKvPool.apply_moves`` does the page copies it decides.
 from __future__ import annotations
 
 import math
+import threading
 from ctypes import addressof, c_int32
 
 import numpy as np
@@ -58,10 +59,21 @@ class RotaryTable:
         return cls(table.contiguous(), sections, interleaved)
 
 
+class _Kept(threading.local):
+    """Workspaces by stream, of one thread: they go with it."""
+
+    def __init__(self):
+        self.by_stream = {}
+
+
 class GqaKvPool:
     """A grouped-head paged cache on one GPU: ``cache``
     ``[n_layers, n_pages, 2 (K, V), n_kv_heads, 64, head_dim]``, bf16 or f16,
-    head_dim 64 or 128.  Storage it makes itself is zeroed."""
+    head_dim 64 or 128.  Storage it makes itself is zeroed.
+
+    Threads may call it side by side.  The attentions' workspaces are kept for
+    each thread and stream that calls without one (up to 39 MB, with the pool
+    or the thread); ``workspace=`` takes the caller's."""
 
     def __init__(self, n_pages: int, n_kv_heads: int, head_dim: int, n_layers: int = 1,
                  dtype: torch.dtype = torch.bfloat16, device: int | str | torch.device | None = None):
@@ -111,7 +123,7 @@ class GqaKvPool:
         self._s = status.data_ptr()
         self._prefill_ws = self.lib.rkv_gqa_prefill_workspace_bytes(self._v)
         self._decode_ws = {}  # bytes by number of q heads: they do not grow with the sequences
-        self._kept = {}  # workspaces by stream
+        self._kept = _Kept()
         self._scale = 1.0 / math.sqrt(self.head_dim)
 
     # -- status ---------------------------------------------------------------
@@ -164,8 +176,9 @@ class GqaKvPool:
         return out, self._need(out, self.dtype, name, shape)
 
     def _workspace(self, workspace: torch.Tensor | None, nbytes: int, stream, handle: int) -> torch.Tensor:
-        """The caller's workspace, or one that the pool keeps for the current stream (a call on it comes after the one
-        before); with a stream given, or in a graph's capture, memory of the call's own."""
+        """The caller's workspace, or one that the pool keeps for this thread and the current stream (of a thread's calls
+        on a stream each comes after the one before; another thread's two launches may fall between a call's own);
+        with a stream given, or in a graph's capture, memory of the call's own."""
         if workspace is not None:
             if workspace.get_device() != self._index or not workspace.is_contiguous() or \
                     workspace.numel() * workspace.element_size() < nbytes:
@@ -176,9 +189,10 @@ class GqaKvPool:
                 return torch.empty(nbytes, dtype=torch.uint8, device=self.device)
         if torch.cuda.is_current_stream_capturing():
             return torch.empty(nbytes, dtype=torch.uint8, device=self.device)
-        kept = self._kept.get(handle)
+        by_stream = self._kept.by_stream
+        kept = by_stream.get(handle)
         if kept is None or kept.numel() < nbytes:
-            kept = self._kept[handle] = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+            kept = by_stream[handle] = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
         return kept
 
     def _stream(self, stream) -> int:

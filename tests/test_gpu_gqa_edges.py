@@ -1,5 +1,7 @@
 """More of the grouped-head paged cache on the GPU: what only shows over many steps, at the ends of the arguments'
 ranges, with values that are not finite, and from several threads."""
+import threading
+
 import pytest
 import torch
 
@@ -41,3 +43,41 @@ def test_widest_windows(cuda, op, window):
         out = pool.decode(0, b.q, b.table, b.kv_lens, window=window)
     pool.check(op)
     close(out, *b.want(window=window), BF)
+
+
+# ---------------------------------------------------------------- threads
+@pytest.mark.parametrize("op", ["prefill", "decode"])
+def test_two_threads_on_one_stream(cuda, op):
+    """Both queue calls whose rows are shared out and joined, on the default stream; each gets its own results."""
+    batches = [Batch([1] * 3 if op == "decode" else [3, 20, 1], lens, 8, 2, 128, BF, seed=33 + i)
+               for i, lens in enumerate(([3000, 7000, 900], [9000, 400, 2500]))]
+    cache = torch.cat([b.cache for b in batches], dim=1)
+    tables = [batches[0].table, torch.where(batches[1].table >= 0, batches[1].table + batches[0].cache.shape[1], -1)]
+    pool = GqaKvPool.over(cache)
+
+    def call(i):
+        b = batches[i]
+        if op == "decode":
+            return pool.decode(0, b.q, tables[i], b.kv_lens)
+        return pool.prefill(0, b.q, b.cu_q, tables[i], b.kv_lens)
+
+    alone = [call(i) for i in range(2)]
+    for out, b in zip(alone, batches):
+        close(out, *b.want(), BF)
+    torch.cuda.synchronize()
+    results = [[], []]
+    start = threading.Barrier(2)
+
+    def work(i):
+        start.wait()
+        for _ in range(300):
+            results[i].append(call(i))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    pool.check(op)
+    for i in range(2):
+        assert len(results[i]) == 300 and all(torch.equal(r, alone[i]) for r in results[i])
