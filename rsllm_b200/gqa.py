@@ -8,6 +8,7 @@ cache; ``GqaKvPool.apply_moves`` does the page copies it decides.
 """
 from __future__ import annotations
 
+import functools
 import math
 import threading
 from ctypes import addressof, c_int32
@@ -21,6 +22,9 @@ from .kvcache import CudaError, InvalidArgument, ShapeMismatch, check, raise_sta
 
 # The current stream's handle without a Stream object around it, where this torch has it.
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+# The current device without torch.cuda.current_device's check that CUDA is initialised (a pool's tensors are on it).
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 _DTYPES = {torch.bfloat16: _abi.GQA_BF16, torch.float16: _abi.GQA_F16}
 
@@ -59,6 +63,19 @@ class RotaryTable:
         return cls(table.contiguous(), sections, interleaved)
 
 
+def _on_its_device(method):
+    """The library launches on the current device: for the call, that is the pool's."""
+
+    @functools.wraps(method)
+    def call(self, *args, **kwargs):
+        if _current_device() == self._index:
+            return method(self, *args, **kwargs)
+        with torch.cuda.device(self._index):
+            return method(self, *args, **kwargs)
+
+    return call
+
+
 class _Kept(threading.local):
     """Workspaces by stream, of one thread: they go with it."""
 
@@ -71,7 +88,8 @@ class GqaKvPool:
     ``[n_layers, n_pages, 2 (K, V), n_kv_heads, 64, head_dim]``, bf16 or f16,
     head_dim 64 or 128.  Storage it makes itself is zeroed.
 
-    Threads may call it side by side.  The attentions' workspaces are kept for
+    Calls run on the cache's device, whichever is current, on its current
+    stream or ``stream``.  Threads may call it side by side.  The attentions' workspaces are kept for
     each thread and stream that calls without one (up to 39 MB, with the pool
     or the thread); ``workspace=`` takes the caller's."""
 
@@ -197,11 +215,14 @@ class GqaKvPool:
 
     def _stream(self, stream) -> int:
         if stream is not None:
+            if stream.device_index != self._index:
+                raise InvalidArgument(f"stream: expected one of {self.device}")
             return stream.cuda_stream
         return _raw_stream(self._index) if _raw_stream is not None else \
             torch.cuda.current_stream(self.device).cuda_stream
 
     # -- append -------------------------------------------------------------------
+    @_on_its_device
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, slot_mapping: torch.Tensor,
                q: torch.Tensor | None = None, rotary: RotaryTable | None = None, pos: torch.Tensor | None = None,
                q_out: torch.Tensor | None = None, stream: torch.cuda.Stream | None = None) -> torch.Tensor | None:
@@ -239,6 +260,7 @@ class GqaKvPool:
         return q_out if q is not None else None
 
     # -- attention -----------------------------------------------------------------
+    @_on_its_device
     def prefill(self, layer: int, q: torch.Tensor, cu_q: torch.Tensor, page_table: torch.Tensor, kv_lens: torch.Tensor,
                 softmax_scale: float | None = None, window: int = 0, sinks: torch.Tensor | None = None,
                 out: torch.Tensor | None = None, workspace: torch.Tensor | None = None,
@@ -264,6 +286,7 @@ class GqaKvPool:
             check(rc, "prefill")
         return out
 
+    @_on_its_device
     def decode(self, layer: int, q: torch.Tensor, page_table: torch.Tensor, kv_lens: torch.Tensor,
                softmax_scale: float | None = None, window: int = 0, sinks: torch.Tensor | None = None,
                out: torch.Tensor | None = None, workspace: torch.Tensor | None = None,
@@ -289,6 +312,7 @@ class GqaKvPool:
         return out
 
     # -- page moves ------------------------------------------------------------------
+    @_on_its_device
     def copy_pages(self, src: torch.Tensor, dst: torch.Tensor, stream: torch.cuda.Stream | None = None) -> None:
         """Every layer: page dst[i] <- page src[i] (int32; disjoint sets)."""
         n = src.shape[0] if src.dim() == 1 else -1
@@ -296,6 +320,7 @@ class GqaKvPool:
                                           self._need(dst, torch.int32, "dst", (n,)), n, self._s,
                                           self._stream(stream)), "copy_pages")
 
+    @_on_its_device
     def apply_moves(self, src, dst, stream: torch.cuda.Stream | None = None) -> None:
         """Applies a plan-only pool's page moves (``PrefixKvPool.take_moves``,
         host arrays) in their order: as few ``copy_pages`` calls as keep a page

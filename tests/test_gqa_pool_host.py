@@ -42,9 +42,11 @@ class Lib:
 
 @pytest.fixture
 def make(monkeypatch):
-    """make(during): (pool, decode, prefill); ``make.stream`` is the current stream's handle."""
-    state = type("State", (), {"stream": 0})()
+    """make(during): (pool, decode, prefill); ``make.state`` holds the current stream's handle and the current device
+    (CPU tensors are on "device" -1)."""
+    state = type("State", (), {"stream": 0, "device": -1})()
     monkeypatch.setattr(gqa, "_raw_stream", lambda index: state.stream)
+    monkeypatch.setattr(gqa, "_current_device", lambda: state.device)
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
 
     def build(during):
@@ -104,3 +106,60 @@ def test_a_thread_keeps_one_workspace_a_stream(make):
     make.state.stream = 0
     decode()
     assert seen[6] == (0, first)
+
+
+def test_calls_run_on_the_pools_device(make, monkeypatch):
+    """With another device current, every call makes the pool's own current until it is back: the library launches,
+    and a capture is asked about, on the current one."""
+    calls = []
+    pool, decode, prefill = make(lambda name, workspace, stream: calls.append((name, make.state.device)))
+
+    class Guard:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            self.before, make.state.device = make.state.device, self.index
+
+        def __exit__(self, *exc):
+            make.state.device = self.before
+
+    def capturing():
+        calls.append(("capturing", make.state.device))
+        return False
+
+    monkeypatch.setattr(torch.cuda, "device", Guard)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", capturing)
+    k = torch.zeros((1, 2, 64), dtype=BF)
+    one = torch.tensor([1], dtype=torch.int32)
+    for current in (-1, 3):
+        make.state.device = current
+        calls.clear()
+        decode()
+        prefill()
+        pool.append(0, k, k, one)
+        pool.copy_pages(one, one)
+        pool.apply_moves([1, 1], [2, 3])
+        assert {name for name, _ in calls} == {"decode", "prefill", "append", "copy", "capturing"}
+        assert all(device == -1 for _, device in calls), calls
+        assert make.state.device == current
+        with pytest.raises(rk.ShapeMismatch):  # and after an error
+            pool.append(0, k[:, :1], k, one)
+        assert make.state.device == current
+
+
+def test_a_stream_of_another_device_is_refused(make):
+    calls = []
+    pool, *_ = make(lambda *a: calls.append(a))
+    k = torch.zeros((1, 2, 64), dtype=BF)
+    q = torch.zeros((1, 4, 64), dtype=BF)
+    one = torch.tensor([1], dtype=torch.int32)
+    table = torch.zeros((1, 2), dtype=torch.int32)
+    cu = torch.tensor([0, 1], dtype=torch.int32)
+    other = type("Stream", (), {"device_index": 1, "cuda_stream": 5})()
+    for call in (lambda: pool.append(0, k, k, one, stream=other), lambda: pool.copy_pages(one, one, stream=other),
+                 lambda: pool.decode(0, q, table, one, stream=other),
+                 lambda: pool.prefill(0, q, cu, table, one, stream=other)):
+        with pytest.raises(rk.InvalidArgument):
+            call()
+    assert not calls
