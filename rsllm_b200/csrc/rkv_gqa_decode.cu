@@ -479,7 +479,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) decode_kernel(const Para
             const float sink = sink_log2(p.sinks, head0 + r);
             const float top = fmaxf(M, sink);
             const float w = ex2(M - top);
-            return M == -INFINITY ? 0.f : w / (l * w + ex2(sink - top));
+            return M == -INFINITY && l == 0.f ? 0.f : w / (l * w + ex2(sink - top));
           };
           const float n0 = r0 < live ? norm(r0, M0, L0) : 0.f, n1 = r0 + 8 < live ? norm(r0 + 8, M1, L1) : 0.f;
           uint16_t* d0 = p.out + ((int64_t)s * p.n_q_heads + head0 + r0) * D + 2 * t4;
@@ -563,7 +563,7 @@ __global__ void __launch_bounds__(kWarps == 1 ? kJoinThreads : 32 * kWarps) join
     }
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
-      if (e[k].x == -INFINITY) continue;
+      if (e[k].x == -INFINITY && e[k].y == 0.f) continue;  // nothing there (a sum of NaN is something)
       const float top = fmaxf(m, e[k].x);
       const float a = ex2(m - top), w = ex2(e[k].x - top);  // 0 from -inf
       l = l * a + w * e[k].y;

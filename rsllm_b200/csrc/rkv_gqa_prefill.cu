@@ -761,7 +761,8 @@ prefill_kernel(const Params p, const __grid_constant__ CUtensorMap map, const __
       if (lane == 0) mbar_arrive(job_free);
       const int token = t * p.tile_tokens + row / p.group;
       const bool live = row < used && token < w.tokens;
-      const bool seen = m != -INFINITY;  // a row that saw nothing: zeros, whatever O holds
+      // a row that saw nothing: zeros, whatever O holds; one that saw nothing but NaN has a sum of NaN, and is not such a row
+      const bool seen = m != -INFINITY || l != 0.f;
       const int head = w.head * p.group + row % p.group;
       float f = seen ? 1.f : 0.f;
       const int64_t at = (int64_t)w.slot * kBlockRows + t * kM + row;
@@ -886,7 +887,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p) {
     }
 #pragma unroll
     for (int k = 0; k < kMine; ++k) {
-      if (e[k].x == -INFINITY) continue;  // it saw nothing there, and wrote no O
+      if (e[k].x == -INFINITY && e[k].y == 0.f) continue;  // it saw nothing there, and wrote no O
       const float top = fmaxf(m[k], e[k].x);
       const float a = ex2(m[k] - top), w = ex2(e[k].x - top);  // 0 from -inf
       l[k] = l[k] * a + e[k].y * w;

@@ -81,3 +81,40 @@ def test_two_threads_on_one_stream(cuda, op):
     pool.check(op)
     for i in range(2):
         assert len(results[i]) == 300 and all(torch.equal(r, alone[i]) for r in results[i])
+
+
+# ------------------------------------------------------------------- NaN
+@pytest.mark.parametrize("kv", [1, 40, 700, 9000])
+@pytest.mark.parametrize("d,dtype", [(128, BF), (64, HF)])
+@pytest.mark.parametrize("op", ["prefill", "decode"])
+def test_nan_is_not_taken_for_an_empty_row(cuda, op, d, dtype, kv):
+    """A q row, or every K row that a token sees, of NaN: the result is NaN, not the zeros of a token that sees nothing,
+    with rows shared out or not, with sinks or not; every other result keeps its bits."""
+    q_lens = [1, 1, 1] if op == "decode" else [min(kv, 30), 5, 1]
+    b = Batch(q_lens, [kv, 300, 0], 8, 2, d, dtype, seed=35)
+    pool = GqaKvPool.over(b.cache)
+
+    def call(q, sinks):
+        if op == "decode":
+            return pool.decode(0, q, b.table, b.kv_lens, sinks=sinks)
+        return pool.prefill(0, q, b.cu_q, b.table, b.kv_lens, sinks=sinks)
+
+    for sinks in (None, b.sinks):
+        clean = call(b.q, sinks)
+        close(clean, *b.want(sinks=sinks is not None), dtype)
+        q = b.q.clone()
+        q[0, 5] = float("nan")
+        out = call(q, sinks)
+        assert out[0, 5].isnan().all()
+        out[0, 5] = clean[0, 5]
+        assert torch.equal(out, clean)
+        # row 0 of kv head 1 in the first sequence: the tokens that see no other row see nothing else
+        page = int(b.table[0, 0])
+        kept = b.cache[0, page, 0, 1].clone()
+        b.cache[0, page, 0, 1, 0] = float("nan")
+        out = call(b.q, sinks)
+        b.cache[0, page, 0, 1] = kept
+        assert out[:q_lens[0], 4:].isnan().all()
+        out[:q_lens[0], 4:] = clean[:q_lens[0], 4:]
+        assert torch.equal(out, clean)
+        pool.check(op)
