@@ -768,7 +768,9 @@ RKV_API rkv_status rkv_gqa_prefill(const rkv_gqa_view* cache, int32_t layer, con
  * at position kv_lens[s] - 1; a sequence of no rows gives zeros), the rows
  * divided evenly over the GPU whatever the lengths and joined through workspace
  * (rkv_gqa_decode_workspace_bytes bytes of device memory, 16-byte aligned; its
- * contents need no initialisation and do not outlast the call). */
+ * contents need no initialisation and do not outlast the call).  Its weights
+ * meet V as two terms of the cache's type, which together hold 16 (bf16) or 22
+ * bits of them. */
 RKV_API int64_t rkv_gqa_decode_workspace_bytes(const rkv_gqa_view* cache, int32_t n_seq, int32_t n_q_heads);
 RKV_API rkv_status rkv_gqa_decode(const rkv_gqa_view* cache, int32_t layer, const void* q, int64_t q_token_stride,
                                   int64_t q_head_stride, int32_t n_seq, int32_t n_q_heads, const int32_t* page_table,

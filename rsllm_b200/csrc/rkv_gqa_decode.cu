@@ -24,16 +24,20 @@
 //   * The products are mma.sync m16n8k16 with the group's q heads (16 at a
 //     time) as rows: S = Q K^T from ldmatrix, P stays in registers as the A
 //     operand of O += P V (ldmatrix.trans).  Rows past the group are zero: the
-//     tensor cores have time for them.
+//     tensor cores have time for them.  They have time for the weights twice,
+//     too: rounded to the cache's type, and then what that rounding left of them,
+//     so that the result is as good as with weights of 32 bits (without the
+//     second product its error against 64 bits was 1.1 to 1.45 times as large;
+//     it costs 1% of the 64-sequence time below, and the ragged one nothing).
 //
 // Groups of more than 16 q heads are taken 16 at a time, each reading the
 // pages again (from L2 when their CTAs run together).
 //
-// Measured: 64 sequences of 32768 rows, 32 q and 8 kv heads of 128, bf16: 1.255 ms,
-// 6.85 TB/s (a copy, which also writes, reaches 6.47).  One sequence of 131072
-// rows and 2 kv heads: 30.6 us, of which 5 pass before the first page is there
-// and 5 in the join; 256 ragged ones of up to 4096 rows, 4 kv heads of 64, f16: 137
-// us, 5.8 TB/s.
+// Measured: 64 sequences of 32768 rows, 32 q and 8 kv heads of 128, bf16: 1.28 ms,
+// 6.7 TB/s (a copy, which also writes, reaches 6.47).  One sequence of 131072
+// rows and 2 kv heads: 31.0 us, of which 5 pass before the first page is there
+// and 5 in the join; 256 ragged ones of up to 4096 rows, 4 kv heads of 64, f16: 133
+// to 138 us, 5.8 to 6 TB/s.
 #include "rkv_gqa.cuh"
 #include "rkv_gqa_plan.h"
 
@@ -393,7 +397,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) decode_kernel(const Para
           }
         }
         const float s0 = m0 == -INFINITY ? 0.f : m0, s1 = m1 == -INFINITY ? 0.f : m1;  // nothing seen yet: weights 0
-        uint32_t pf[4];
+        uint32_t pf[4], pr[4];  // the weights in the type, and what that rounding left of them
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           const float e0 = ex2(x[j][0] - s0), e1 = ex2(x[j][1] - s0), e2 = ex2(x[j][2] - s1), e3 = ex2(x[j][3] - s1);
@@ -401,6 +405,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) decode_kernel(const Para
           l1 += e2 + e3;
           pf[2 * j] = T::pack(e0, e1);
           pf[2 * j + 1] = T::pack(e2, e3);
+          const float2 h0 = T::unpack(pf[2 * j]), h1 = T::unpack(pf[2 * j + 1]);
+          pr[2 * j] = T::pack(e0 - h0.x, e1 - h0.y);
+          pr[2 * j + 1] = T::pack(e2 - h1.x, e3 - h1.y);
         }
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) {
@@ -408,6 +415,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) decode_kernel(const Para
           ldsm4t(vs + sw_off(vrow, 2 * i + vchunk), b);
           mma<T>(o[2 * i], pf, b[0], b[1]);
           mma<T>(o[2 * i + 1], pf, b[2], b[3]);
+          mma<T>(o[2 * i], pr, b[0], b[1]);
+          mma<T>(o[2 * i + 1], pr, b[2], b[3]);
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(bars + 8 * (kStages + st));

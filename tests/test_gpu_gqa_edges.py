@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from rsllm_b200 import GqaKvPool
-from tests.gqa_cases import Batch, close
+from tests.gqa_cases import UNIT, Batch, close
 
 pytestmark = pytest.mark.gpu
 
@@ -118,3 +118,21 @@ def test_nan_is_not_taken_for_an_empty_row(cuda, op, d, dtype, kv):
         out[:q_lens[0], 4:] = clean[:q_lens[0], 4:]
         assert torch.equal(out, clean)
         pool.check(op)
+
+
+# ------------------------------------------------------------- the weights
+@pytest.mark.parametrize("hq,hkv,d,dtype,sinks", [(16, 2, 128, BF, False), (8, 8, 64, BF, True), (34, 2, 128, HF, False),
+                                                  (4, 4, 64, HF, True)])
+def test_decode_weights_keep_their_bits(cuda, hq, hkv, d, dtype, sinks):
+    """Few rows, so that their weights are large and their errors do not average out.  The weights' two terms hold them
+    to 2^-16, the exponentials and logits are good to 2^-13 each in numerator and denominator (2^-12 sum w |v| in
+    all), and the output is rounded once (u |out|); 1e-6 for f16 results near the subnormals.  One term would
+    add u sum w |v|."""
+    kv_lens = [1, 2, 3, 4, 5, 7, 9, 16, 17, 33, 64, 65, 100, 900]
+    b = Batch([1] * len(kv_lens), kv_lens, hq, hkv, d, dtype, seed=36)
+    pool = GqaKvPool.over(b.cache)
+    out = pool.decode(0, b.q, b.table, b.kv_lens, sinks=b.sinks if sinks else None).double().cpu()
+    pool.check("decode")
+    want, mag = b.want(sinks=sinks)
+    over = (out - want).abs() - ((2.0 ** -12 + 2.0 ** -16) * mag + UNIT[dtype] * want.abs() + 1e-6)
+    assert over.max().item() <= 0, f"off by {over.max().item():.3g} more than the bound"
