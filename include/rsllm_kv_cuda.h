@@ -679,7 +679,7 @@ RKV_API rkv_status rkv_indexer_topk_f32(const float* rows, const int64_t* row_st
  * Rows of q, k and v are given as a pointer, a token stride and a head stride
  * in elements (the head_dim elements of a row are contiguous), so that views
  * of one fused projection need no copy: pointers 16-byte aligned, strides
- * multiples of 8.  n_q_heads is a multiple of n_kv_heads, at most 64 times as
+ * multiples of 8 (0, of a broadcast view, in all but rkv_gqa_prefill's q).  n_q_heads is a multiple of n_kv_heads, at most 64 times as
  * many; q head h reads kv head h / (n_q_heads / n_kv_heads). */
 #define RKV_GQA_BF16 0
 #define RKV_GQA_F16 1

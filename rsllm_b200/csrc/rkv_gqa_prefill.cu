@@ -981,6 +981,11 @@ extern "C" rkv_status rkv_gqa_prefill(const rkv_gqa_view* cache, int32_t layer, 
   const AttendArgs args = {*cache,     layer,   q,      q_token_stride, q_head_stride, n_tokens, n_q_heads, page_table,
                            pt_stride,  kv_lens, window, sinks,          softmax_scale, out,      d_status};
   if ((st = check_attend(args, what)) != RKV_OK) return st;
+  // q is copied by a tensor map, whose strides are not zero; one that nothing follows may be anything
+  if ((n_tokens > 1 && q_token_stride == 0) || (n_q_heads > 1 && q_head_stride == 0))
+    return fail(RKV_ERR_SHAPE_MISMATCH, "%s: q must not be a broadcast view (a stride of 0)", what);
+  if (n_tokens == 1) q_token_stride = (int64_t)n_q_heads * cache->head_dim;
+  if (n_q_heads == 1) q_head_stride = cache->head_dim;
   if (!cu_q) return fail(RKV_ERR_INVALID_ARGUMENT, "%s: cu_q is required", what);
   if (!workspace || !aligned(workspace, 32) || !aligned(out, 32))
     return fail(RKV_ERR_INVALID_ARGUMENT, "%s: out and a workspace, both 32-byte aligned, are required", what);

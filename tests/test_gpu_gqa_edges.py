@@ -5,6 +5,7 @@ import threading
 import pytest
 import torch
 
+import rsllm_b200 as rk
 from rsllm_b200 import GqaKvPool
 from tests.gqa_cases import UNIT, Batch, close
 
@@ -136,3 +137,22 @@ def test_decode_weights_keep_their_bits(cuda, hq, hkv, d, dtype, sinks):
     want, mag = b.want(sinks=sinks)
     over = (out - want).abs() - ((2.0 ** -12 + 2.0 ** -16) * mag + UNIT[dtype] * want.abs() + 1e-6)
     assert over.max().item() <= 0, f"off by {over.max().item():.3g} more than the bound"
+
+
+# ---------------------------------------------------------------- strides
+def test_broadcast_q_k_and_v(cuda):
+    """One q row for every sequence, and one k and v row for every token, as expanded views: decode and append take
+    them as they are, prefill refuses them."""
+    b = Batch([1] * 3, [70, 1, 300], 8, 2, 128, BF, seed=37)
+    pool = GqaKvPool.over(b.cache)
+    q = b.q[:1].expand(3, 8, 128)
+    assert torch.equal(pool.decode(0, q, b.table, b.kv_lens), pool.decode(0, q.contiguous(), b.table, b.kv_lens))
+    with pytest.raises(rk.ShapeMismatch):
+        pool.prefill(0, q, b.cu_q, b.table, b.kv_lens)
+    one = pool.prefill(0, b.q[:1], b.cu_q[:2], b.table[:1], b.kv_lens[:1])
+    row = torch.randn((1, 1, 128), device=cuda).to(BF).expand(5, 2, 128)
+    slots = torch.arange(5, dtype=torch.int32, device=cuda) + 64 * int(b.table[2, 4])
+    pool.append(0, row, row, slots)
+    pool.check()
+    assert (b.cache[0, int(b.table[2, 4]), :, :, :5] == row[0, 0]).all()
+    close(one, *[x[:1] for x in b.want()], BF)

@@ -1,12 +1,13 @@
 """GqaKvPool's own bookkeeping, without a GPU: a pool over CPU tensors whose library is a stand-in that records what
 it is given."""
 import threading
+from ctypes import addressof
 
 import pytest
 import torch
 
 import rsllm_b200 as rk
-from rsllm_b200 import gqa
+from rsllm_b200 import _abi, gqa
 
 BF = torch.bfloat16
 
@@ -163,3 +164,17 @@ def test_a_stream_of_another_device_is_refused(make):
         with pytest.raises(rk.InvalidArgument):
             call()
     assert not calls
+
+
+def test_prefill_refuses_a_broadcast_q():
+    """A stride of 0 between tokens or heads, before anything is launched; with one of them it is of no use."""
+    base = 0x100000
+    view = _abi.GqaView(base, 8, 2, 2, 128, _abi.GQA_BF16)
+
+    def prefill(n, heads, ts, hs, cu=base):
+        return _abi.load().rkv_gqa_prefill(addressof(view), 0, base, ts, hs, n, heads, cu, 1, base, 4, base, 0, 0, 0.1,
+                                           base, base, 0, 0)
+
+    assert prefill(2, 8, 0, 128) == _abi.RKV_ERR_SHAPE_MISMATCH
+    assert prefill(2, 8, 1024, 0) == _abi.RKV_ERR_SHAPE_MISMATCH
+    assert prefill(1, 8, 0, 128, cu=0) == _abi.RKV_ERR_INVALID_ARGUMENT  # refused for its offsets only
