@@ -418,6 +418,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) decode_kernel(const Para
           mma<T>(o[2 * i], pr, b[0], b[1]);
           mma<T>(o[2 * i + 1], pr, b[2], b[3]);
         }
+        // This warp's reads of the stage come before the copy that overwrites it.  The barrier alone orders them among loads
+        // and stores, not with the copies of the other proxy: without the fence a copy that came at once (pages in L2,
+        // launches close behind one another) overtook the last reads of V, once in some hundred to thousand launches.
+        fence_proxy_async();
         __syncwarp();
         if (lane == 0) mbar_arrive(bars + 8 * (kStages + st));
       }

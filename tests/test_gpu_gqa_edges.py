@@ -1,5 +1,6 @@
 """More of the grouped-head paged cache on the GPU: what only shows over many steps, at the ends of the arguments'
 ranges, with values that are not finite, and from several threads."""
+import random
 import threading
 
 import pytest
@@ -156,3 +157,29 @@ def test_broadcast_q_k_and_v(cuda):
     pool.check()
     assert (b.cache[0, int(b.table[2, 4]), :, :, :5] == row[0, 0]).all()
     close(one, *[x[:1] for x in b.want()], BF)
+
+
+# ------------------------------------------------------------- the ring
+@pytest.mark.parametrize("n,least,most,hq,hkv,d,dtype,window", [
+    (9, 626, 5713, 40, 8, 64, HF, 0),
+    (30, 0, 4110, 4, 4, 64, HF, 0),
+    (35, 71, 1602, 28, 4, 64, BF, 0),
+    (30, 0, 27158, 8, 8, 64, BF, 1024),
+    (36, 0, 4379, 4, 4, 128, BF, 1024),
+])
+def test_decode_repeats_itself_close_behind(cuda, n, least, most, hq, hkv, d, dtype, window):
+    """Launches close behind one another, their pages in L2, so that a page is overwritten as soon as it may be: every
+    one gives the same bits."""
+    r = random.Random(7)
+    kv_lens = [most if i == 0 else r.randint(least, most) for i in range(n)]
+    b = Batch([1] * n, kv_lens, hq, hkv, d, dtype, seed=38)
+    pool = GqaKvPool.over(b.cache)
+    first = pool.decode(0, b.q, b.table, b.kv_lens, window=window)
+    close(first, *b.want(window=window), dtype)
+    other = torch.zeros(1, dtype=torch.int64, device=cuda)
+    for _ in range(100):
+        torch.cuda._sleep(2_000_000)  # the launches queue up behind it
+        for out in [pool.decode(0, b.q, b.table, b.kv_lens, window=window) for _ in range(40)]:
+            other += (out != first).any()
+    pool.check("decode")
+    assert int(other) == 0
