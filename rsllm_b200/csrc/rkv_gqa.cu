@@ -134,7 +134,9 @@ struct AppendParams {
 // axes, f16: 76 us, 4.95 TB/s (101 to 133 us where every thread worked out its heads
 // and the axes of its pairs for every token: 67 instead of 41 million instructions).
 // Heads a thread x CTAs an SM: 3 x 4 and 3 x 5 76 us, 3 x 6 82 (spills), 2 x 8 99,
-// 4 x 4 80, 1 x 12 118.
+// 4 x 4 80, 1 x 12 118.  Where a token's heads fill fewer of a CTA's chunks, less is
+// on its way: 20000 tokens of 32 + 8 + 8 heads of 128 reach 5.9 TB/s, of 28 + 4 + 4
+// heads of 64 3.4, of 14 + 2 + 2 of 64 2.2.
 constexpr int kAppendThreads = 128, kAhead = 3, kAppendCtas = 4;
 template <int D>
 struct AppendShape {

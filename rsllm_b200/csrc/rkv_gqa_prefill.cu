@@ -46,7 +46,7 @@
 // they were 350 clocks more a step, and the issuing warp bound the step: 580 us
 // for 8192 tokens.)
 //
-// What bounds a step of both tiles (1750 to 1950 clocks, head_dim 128): 1280 of
+// What bounds a step of both tiles (some 1750 clocks, head_dim 128): 1280 of
 // MMAs -- S with 64 columns reads 6 KB of operands for 32 clocks of products, the
 // shared memory's 128 bytes a clock make it 48 -- and a chain of the softmax
 // warps: 150 for the barrier of S, 80 to 110 for loads, 160 to 250 for maxima and
